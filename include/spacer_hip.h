@@ -472,6 +472,80 @@ int spacer_attn_fwd_pair(const void* q_hi, const void* q_lo, const void* k_hi, c
 /* variant: 0 = DMA-staged tiles, 256 query rows per workgroup (round 5); 1 = the register-staged round-3 kernel (A/B runs, tests).
  * Same MFMA order per wave: the two give the same bits. */
 
+/* ------------------------------------------------------------------------------------------------
+ * The rollout's key/value cache in 16 or 8 bits, and the attention that reads it (what HF generate's DynamicCache and the attention of its
+ * decode loop do behind TR:463; a vLLM engine's kv_cache_dtype, vllm_grpo_trainer_modified.py:344).
+ * A cache holds n_seq sequences x capacity positions x kv_heads rows of head_dim numbers (64 or 128), the last dimension contiguous, the
+ * others at any strides (in elements) whose rows start at multiples of 16 bytes; k and v share them.  8-bit rows carry one fp32 scale each
+ * (strides in floats) and stand for code * scale:
+ *   SPACER_KV_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| / scale <= 448
+ *   SPACER_KV_INT8  two's complement codes -127 .. 127; scale = max|x| / 127 in fp32, ties of x / scale to even
+ * A row with a NaN or an infinity gets scale NaN and codes 0 (it stands for NaN).
+ * ---------------------------------------------------------------------------------------------- */
+enum spacer_kv_format { SPACER_KV_BF16 = 0, SPACER_KV_E4M3 = 1, SPACER_KV_INT8 = 2 };
+typedef struct spacer_kv_cache {
+    int struct_bytes; /* = sizeof(spacer_kv_cache) as the CALLER declares it; any other value is SPACER_EINVAL */
+    int format;       /* enum spacer_kv_format */
+    int n_seq, capacity, kv_heads, head_dim;
+    void* k;
+    void* v;
+    float* k_scale; /* NULL for SPACER_KV_BF16 */
+    float* v_scale;
+    long stride_seq, stride_head, stride_pos;
+    long scale_stride_seq, scale_stride_head, scale_stride_pos;
+} spacer_kv_cache;
+
+/* Slot (sequence, position) takes the source row rows[sequence * capacity + position] of k / v (bf16 [n_src, kv_heads * head_dim], row
+ * stride ld elements, 16-byte aligned rows); a value below 0 or >= n_src leaves the slot as it is.  Several slots may name one row. */
+int spacer_kv_write(const spacer_kv_cache* cache, const void* k, const void* v, long ld, int n_src, const int* rows, spacer_stream_t stream);
+/* Row s * N + i of k / v goes to position len[s] + i of sequence s (len: one value for all sequences, or with len_per_seq != 0 one each;
+ * device memory, so that the step can be replayed from a hipGraph).  Positions outside the cache are dropped. */
+int spacer_kv_append(const spacer_kv_cache* cache, const void* k, const void* v, long ld, int N, const int* len, int len_per_seq,
+                     spacer_stream_t stream);
+/* k_out / v_out [n_seq, capacity, kv_heads, head_dim] (fp32, or bf16: e4m3 values are exact there, int8 values are rounded once) = the values the
+ * cache stands for; with len (int32 [n_seq], or NULL) the positions at and behind len[s] are zero. */
+int spacer_kv_read(const spacer_kv_cache* cache, const int* len, void* k_out, void* v_out, int out_f32, spacer_stream_t stream);
+/* spacer_decode_qkv_finish (rowss NULL) / spacer_decode_qkv_finish_normed with K and V going to position tail_len of the cache's sequences
+ * (cache->n_seq = the batch), rounded to bf16 first, then to the cache's format as spacer_kv_append rounds. */
+int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, const float* cos_t, const float* sin_t, void* q_out,
+                                   const spacer_kv_cache* cache, const int* tail_len, int len_per_seq, const float* rowss, float* rowss_zero,
+                                   int norm_cols, float eps, int Hq, spacer_stream_t stream);
+
+/* Decode attention over such caches, for one new token per sequence or a tree of N drafted ones (N <= 64; q row b * N + i = node i of
+ * sequence b, bf16 [B * N, Hq * head_dim] with row stride q_ld).  Node i sees
+ *   the positions [0, prompt_len[p]) of its prompt p in `prompt` (shared by the prompt's sequences; NULL: no prompt),
+ *   the positions [0, tail_len[b]) of sequence b in `tail` (NULL: none), and
+ *   the nodes j whose bit j is set in tree[b * tree_per_seq * N + i] (int64; NULL: j <= i), node j at position tail_len[b] + j of `tail`.
+ * Prompt p owns the sequences [row0[p], row0[p + 1]) (int32 [n_prompts + 1] on the device, ascending), or with row0 NULL
+ * [p * rows, (p + 1) * rows); at most `rows` of them.  Lengths are clamped to the caches.  A node that sees nothing gets zeros.
+ * o bf16 [B * N, Hq * head_dim] contiguous.  prompt and tail share format, kv_heads and head_dim; tail->n_seq = B.
+ * workspace: spacer_attn_cache_workspace_bytes(...) bytes of device memory, 16-byte aligned, no initialisation; the cache structs may be NULL
+ * there as in the call.  Launches that share a workspace must be ordered on one stream. */
+long spacer_attn_cache_workspace_bytes(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq);
+int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache* prompt, const int* prompt_len, const int* row0, int rows,
+                      const spacer_kv_cache* tail, const int* tail_len, int len_per_seq, const int64_t* tree, int tree_per_seq, void* o, int B,
+                      int N, int Hq, float scale, void* workspace, long workspace_bytes, spacer_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Logits of one decode step before the sampler (HF generate's RepetitionPenaltyLogitsProcessor, SequenceBiasLogitsProcessor and
+ * PrefixConstrainedLogitsProcessor behind TR:463; presence / frequency penalties, logit_bias and guided decoding of a vLLM engine).
+ * History of a row: `seen` int32 [B, ceil(vocab / 32)], bit v % 32 of word v / 32 = token v has occurred (prompt or completion);
+ * `counts` int32 [B, vocab] = its occurrences in the completion.  Both zeroed by the caller at the start.
+ * ---------------------------------------------------------------------------------------------- */
+/* Marks ids[b * ld + i], i < n (and i < len[b] with len != NULL) as seen in row b, and counts them with counts != NULL.  Ids outside
+ * [0, vocab) are skipped. */
+int spacer_token_history_add(int* seen, int* counts, int B, int vocab, const int64_t* ids, long ld, int n, const int* len, spacer_stream_t stream);
+/* out[b, v] (fp32, row stride ld_out; may be the logits themselves) =
+ *     x = logits[b, v];  seen: x > 0 ? x / r : x * r;  x -= frequency * count + presence * (count > 0);  x += bias;  not allowed: -infinity
+ * computed in 64 bits where a penalty applies and rounded once.  r / frequency / presence: a number for all rows, or fp32 [B] where the pointer
+ * is not NULL.  bias fp32 [B, vocab] with row stride ld_bias (0: one row for all), or NULL.  allowed: int32 [n_masks, ceil(vocab / 32)] bit masks
+ * or NULL; row b takes mask allowed_row[b] (int32; a value outside [0, n_masks): no mask), or with allowed_row NULL mask b (n_masks = B) or 0
+ * (n_masks = 1).  A row whose mask allows nothing is all -infinity. */
+int spacer_process_logits(const float* logits, long ld, float* out, long ld_out, int B, int vocab, const int* seen, const int* counts,
+                          float repetition, const float* repetition_dev, float frequency, const float* frequency_dev, float presence,
+                          const float* presence_dev, const float* bias, long ld_bias, const int* allowed, int n_masks, const int* allowed_row,
+                          spacer_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

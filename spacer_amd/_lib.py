@@ -13,6 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspacer_hip.so")
 
 SPACER_ACT_NONE, SPACER_ACT_QUICK_GELU, SPACER_ACT_GELU_ERF, SPACER_ACT_SILU = 0, 1, 2, 3
+SPACER_KV_BF16, SPACER_KV_E4M3, SPACER_KV_INT8 = 0, 1, 2                 # enum spacer_kv_format
 SPACER_PAIR_SWIGLU, SPACER_PAIR_ROPE, SPACER_PAIR_ACT = 2, 3, 4          # enum spacer_pair_epilogue
 
 
@@ -40,7 +41,21 @@ class AttnSegment(C.Structure):
     _fields_ = [("q_start", C.c_int), ("q_len", C.c_int), ("pre_start", C.c_int), ("pre_len", C.c_int)]
 
 
+class KvCache(C.Structure):
+    """include/spacer_hip.h: spacer_kv_cache -- one key/value cache in bf16, e4m3 or int8 rows."""
+    _fields_ = [("struct_bytes", C.c_int), ("format", C.c_int), ("n_seq", C.c_int), ("capacity", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("stride_seq", C.c_long), ("stride_head", C.c_long), ("stride_pos", C.c_long),
+                ("scale_stride_seq", C.c_long), ("scale_stride_head", C.c_long), ("scale_stride_pos", C.c_long)]
+
+    def __init__(self, **fields):
+        super().__init__(**fields)
+        self.struct_bytes = C.sizeof(KvCache)
+
+
 _p, _i, _l, _f, _u64 = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_uint64
+
+_kv = C.POINTER(KvCache)
 
 # name -> argtypes; every entry returns int.  Kept in the order of include/spacer_hip.h.
 SIGNATURES = {
@@ -113,9 +128,16 @@ SIGNATURES = {
     "spacer_norm_f32_pair": [_p, _p, _p, _p, _p, _i, _i, _f, _i, _p, _p, _p],
     "spacer_rope_f32_pair": [_p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _i, _p],
     "spacer_embed_fwd_f32video": [_p, _p, _p, _p, _p, _i, _i, _p],
+    "spacer_kv_write": [_kv, _p, _p, _l, _i, _p, _p],
+    "spacer_kv_append": [_kv, _p, _p, _l, _i, _p, _i, _p],
+    "spacer_kv_read": [_kv, _p, _p, _p, _i, _p],
+    "spacer_decode_qkv_finish_cache": [_p, _p, _p, _p, _p, _kv, _p, _i, _p, _p, _i, _f, _i, _p],
+    "spacer_attn_cache": [_p, _l, _kv, _p, _p, _i, _kv, _p, _i, _p, _i, _p, _i, _i, _i, _f, _p, _l, _p],
+    "spacer_token_history_add": [_p, _p, _i, _i, _p, _l, _i, _p, _p],
+    "spacer_process_logits": [_p, _l, _p, _l, _i, _i, _p, _p, _f, _p, _f, _p, _f, _p, _p, _l, _p, _i, _p, _p],
     "spacer_attn_fwd_pair": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p],
 }
-OTHER_SYMBOLS = ["spacer_last_error", "spacer_version", "spacer_sample_workspace_bytes", "spacer_attn_decode_workspace_bytes", "spacer_gemm_tile", "spacer_gemm_workspace_bytes", "spacer_gemm_swiglu_fused", "spacer_gemm_pair_fused", "spacer_gemm_pair_epilogue_fused", "spacer_resize_workspace_bytes", "spacer_gemm_skinny_swiglu_workspace_bytes"]
+OTHER_SYMBOLS = ["spacer_last_error", "spacer_version", "spacer_sample_workspace_bytes", "spacer_attn_decode_workspace_bytes", "spacer_gemm_tile", "spacer_gemm_workspace_bytes", "spacer_gemm_swiglu_fused", "spacer_gemm_pair_fused", "spacer_gemm_pair_epilogue_fused", "spacer_resize_workspace_bytes", "spacer_gemm_skinny_swiglu_workspace_bytes", "spacer_attn_cache_workspace_bytes"]
 
 _lib = None
 
@@ -157,6 +179,8 @@ def load() -> C.CDLL:
     lib.spacer_resize_workspace_bytes.restype = C.c_long
     lib.spacer_attn_decode_workspace_bytes.argtypes = [_i, _i]
     lib.spacer_attn_decode_workspace_bytes.restype = C.c_long
+    lib.spacer_attn_cache_workspace_bytes.argtypes = [_kv, _kv, _i, _i, _i, _i]
+    lib.spacer_attn_cache_workspace_bytes.restype = C.c_long
     _lib = lib
     return lib
 

@@ -1,0 +1,508 @@
+// Decode attention over bf16 / e4m3 / int8 key-value caches (kv_cache.h): one new token per sequence or a tree of drafted tokens.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i . k_j - m_i),   k_j = s^k_j K_j,  v_j = s^v_j V_j  (codes K, V; row scales s)
+//
+// Columns and rows.  A column is one query (node i of sequence b, head h); the columns of a kv head that read the same keys are the N side of
+// 16x16x32 bf16 matrix products: the prompt's keys meet every (rollout, node, head) column of the prompt at once, a sequence's own keys its
+// (node, head) columns.  The codes become bf16 in registers (e4m3 and int8 numbers are exact in bf16); s^k multiplies the fp32 scores and s^v
+// the fp32 weights before they are rounded to bf16 for the second product, so no scale costs an operation per element.
+//   S^T[key, col] = K . Q^T     A = K rows straight from memory, B = Q fragments
+//   O^T[d, col]  += V^T . P^T   A = V through a wave-private LDS image and the transposing LDS read, B = the weights just computed: the C layout of S^T
+//                               (lane = column, registers = keys) is the B layout of the second product under a permutation of the keys that the
+//                               image's row order repeats, so no lane exchange lies between the two
+// Work split.  Workgroup = (prompt or sequence, kv head, column block of 16 NC, range of keys); its 4 waves take 32-key tiles in turn and never meet
+// inside the loop: the next tile's K, V and scales are requested before the current one is worked on, so 8 waves per CU keep 64 KB in flight (8 bits).
+// The waves' (O, m, l) are joined through LDS, the ranges' through fp32 records and a second small launch.
+#include "kv_cache.h"
+
+namespace {
+
+constexpr int TK = 32;            // keys per wave and step
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnCacheArgs {
+    const bf16_t* q;
+    long q_ld;
+    KvView prompt, tail;
+    const int *prompt_len, *tail_len, *row0;
+    const int64_t* tree;
+    int len_stride, tree_stride;
+    int n_prompts, rows, B, N, Hq, Hkv;
+    int sa, sb, cba, cbb;         // key ranges and column blocks of the prompt and of the sequence role
+    int na;                       // workgroups of the prompt role (a multiple of 8)
+    float scale;
+    float* rec_o;                 // [sa + sb][B * N * Hq][D]
+    float2* rec_ml;               // [sa + sb][B * N * Hq]: maximum (log2 domain) and sum
+    bf16_t* o;
+};
+
+template <int FMT>
+__device__ __forceinline__ bf16x8 codes_to_bf16(uint2 w) {
+    uint32_t o[4];
+    if (FMT == KV_E4M3) {
+        o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, false));
+        o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, true));
+        o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, false));
+        o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, true));
+    } else {
+        const uint32_t a[2] = {w.x, w.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                o[2 * i + j] = pack_bf2((float)(int8_t)((a[i] >> (16 * j)) & 0xffu), (float)(int8_t)((a[i] >> (16 * j + 8)) & 0xffu));
+    }
+    return __builtin_bit_cast(bf16x8, make_uint4(o[0], o[1], o[2], o[3]));
+}
+
+// maximum over the four 16-lane groups (lanes of the same column)
+__device__ __forceinline__ float group_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t w = __float_as_uint(y);
+    const auto b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int FMT, int D, int NC>
+struct Tile {
+    static constexpr int ES = kv_size<FMT>();
+    static constexpr int RB = D * ES;                   // bytes of a row
+    static constexpr int CPR = RB / 16;                 // 16-byte chunks of a row
+    static constexpr int KL = RB / 64;                  // K loads per lane and 16-key fragment
+    static constexpr int VL = TK * CPR / 64;            // V loads per lane
+    static constexpr int STEPS = D / 32;
+    static constexpr int IMG = TK * RB;                 // bytes of a V image
+    // rows that share the 64 LDS banks' 256 bytes take the same chunk order, the next ones another: fragment reads of 16 rows hit all banks once
+    static __device__ __forceinline__ int swz(int row) { return (row / (RB >= 256 ? 1 : 256 / RB)) & (CPR - 1); }
+};
+
+constexpr int lds_bytes(int es, int D, int nc) {
+    const int work = 4 * (TK * D * es + 2 * TK * 4) + (nc > 2 ? nc * (D / 32) * 64 * 16 : 0);
+    const int join = 4 * 16 * (D + 4) * 4 + 4 * 16 * 8;
+    return work > join ? work : join;
+}
+
+// One workgroup's range of keys [t0, t1) (in 32-key tiles) of `total` keys x 16 NC columns from c0 on, and its record.
+//   col_info(c, row, head, node): the query of column c, or false
+//   base: first key that the mask bits speak of (= total where there are none)
+template <int FMT, int D, int NC, class ColInfo>
+__device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const char* vp, const float* ksp, const float* vsp, long s_pos, long c_pos,
+                       int total, int base, int t0, int t1, int c0, int slot, ColInfo col_info) {
+    using T = Tile<FMT, D, NC>;
+    constexpr int DF = D / 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, g = lane >> 4;
+    const long row_b = s_pos * T::ES;
+    const long ncol_all = (long)A.B * A.N * A.Hq;
+    char* vimg = smem + wave * T::IMG;
+    float* sc = (float*)(smem + 4 * T::IMG) + wave * 2 * TK;
+    char* qlds = smem + 4 * (T::IMG + 2 * TK * 4);
+
+    // ---- queries: fragment (cb, step) = for column l15 the 8 numbers that step's slots of lane group g stand for
+    auto q_frag = [&](int cb, int step) -> bf16x8 {
+        int row, head, node;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (col_info(c0 + cb * 16 + l15, row, head, node)) {
+            const int d = T::ES == 2 ? step * 32 + g * 8 : (step >> 1) * 64 + g * 16 + (step & 1) * 8;
+            x = *(const uint4*)(A.q + ((long)row * A.N + node) * A.q_ld + (long)head * D + d);
+        }
+        return __builtin_bit_cast(bf16x8, x);
+    };
+    bf16x8 qreg[NC <= 2 ? NC : 1][T::STEPS];
+    if (NC <= 2) {
+#pragma unroll
+        for (int cb = 0; cb < (NC <= 2 ? NC : 1); ++cb)
+#pragma unroll
+            for (int s = 0; s < T::STEPS; ++s) qreg[cb][s] = q_frag(cb, s);
+    } else {
+        for (int f = wave; f < NC * T::STEPS; f += 4) *(bf16x8*)(qlds + (f * 64 + lane) * 16) = q_frag(f / T::STEPS, f % T::STEPS);
+        __syncthreads();
+    }
+    uint64_t see[NC];                                     // nodes that the column's node sees
+#pragma unroll
+    for (int cb = 0; cb < NC; ++cb) {
+        int row, head, node;
+        see[cb] = 0;
+        if (base < total && col_info(c0 + cb * 16 + l15, row, head, node))
+            see[cb] = A.tree ? (uint64_t)A.tree[(long)row * A.tree_stride + node] : (node >= 63 ? ~0ull : (2ull << node) - 1);
+    }
+    f32x4 oacc[NC][DF];
+    float m_run[NC], l_run[NC];
+#pragma unroll
+    for (int cb = 0; cb < NC; ++cb) {
+        m_run[cb] = -INFINITY; l_run[cb] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DF; ++d) oacc[cb][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    const float kmul = A.scale * LOG2E;
+
+    uint4 kr[2][T::KL], vr[T::VL];
+    float scr = 0.f;
+    auto fetch = [&](int t) {                             // (keys behind the last repeat it: always inside the cache)
+        const int k0 = t * TK, last = total - 1;
+#pragma unroll
+        for (int kf = 0; kf < 2; ++kf) {
+            const char* p = kp + min(k0 + kf * 16 + l15, last) * row_b + g * 16;
+#pragma unroll
+            for (int h = 0; h < T::KL; ++h) kr[kf][h] = *(const uint4*)(p + h * 64);
+        }
+        if (FMT != KV_BF16) scr = (lane < TK ? ksp : vsp)[min(k0 + (lane & 31), last) * c_pos];
+#pragma unroll
+        for (int i = 0; i < T::VL; ++i)
+            vr[i] = *(const uint4*)(vp + min(k0 + lane / T::CPR + i * (64 / T::CPR), last) * row_b + (lane % T::CPR) * 16);
+    };
+
+    if (t0 + wave < t1) fetch(t0 + wave);
+    for (int t = t0 + wave; t < t1; t += 4) {
+        const int k0 = t * TK;
+        const bool edge = k0 + TK > base;                 // some key of the tile is a node or lies behind the last key
+        asm volatile("" ::: "memory");                    // (the previous step's LDS reads stay in front of these writes: LDS is in order)
+        if (FMT != KV_BF16) sc[lane] = lane < TK ? scr * kmul : scr;
+        bool odd_v = false;                               // a NaN or an infinity in a bf16 V row that some columns must not see
+#pragma unroll
+        for (int i = 0; i < T::VL; ++i) {
+            const int row = lane / T::CPR + i * (64 / T::CPR);
+            *(uint4*)(vimg + row * T::RB + (((lane % T::CPR) ^ T::swz(row)) * 16)) = vr[i];
+            if (FMT == KV_BF16 && edge) {
+                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd_v |= amax2(w[e]) >= 0x7f80u;
+            }
+        }
+        // ---- S^T = K . Q^T
+        f32x4 st[NC][2];
+#pragma unroll
+        for (int cb = 0; cb < NC; ++cb) st[cb][0] = st[cb][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < T::STEPS; ++s) {
+            bf16x8 kf8[2];
+#pragma unroll
+            for (int kf = 0; kf < 2; ++kf) {
+                if (FMT == KV_BF16) kf8[kf] = __builtin_bit_cast(bf16x8, kr[kf][s]);
+                else {
+                    const uint4 x = kr[kf][s >> 1];
+                    kf8[kf] = codes_to_bf16<FMT>((s & 1) ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
+                }
+            }
+#pragma unroll
+            for (int cb = 0; cb < NC; ++cb) {
+                const bf16x8 qf = NC <= 2 ? qreg[NC <= 2 ? cb : 0][s] : *(const bf16x8*)(qlds + ((cb * T::STEPS + s) * 64 + lane) * 16);
+                st[cb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[0], qf, st[cb][0], 0, 0, 0);
+                st[cb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[1], qf, st[cb][1], 0, 0, 0);
+            }
+        }
+        if (t + 4 < t1) fetch(t + 4);                     // the registers of K and V are free: the next tile is under way during the rest
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // image and scales complete before any lane reads them
+        __builtin_amdgcn_wave_barrier();
+        float ksv[2][4], vsv[2][4];
+        if (FMT != KV_BF16) {
+#pragma unroll
+            for (int kf = 0; kf < 2; ++kf) {
+                const float4 a = *(const float4*)(sc + kf * 16 + g * 4), b = *(const float4*)(sc + TK + kf * 16 + g * 4);
+                ksv[kf][0] = a.x; ksv[kf][1] = a.y; ksv[kf][2] = a.z; ksv[kf][3] = a.w;
+                vsv[kf][0] = b.x; vsv[kf][1] = b.y; vsv[kf][2] = b.z; vsv[kf][3] = b.w;
+            }
+        }
+        // ---- online softmax in the log2 domain; the running maximum follows only in steps of more than 2^8 (weights stay below 2^8, far
+        //      inside fp32 and bf16), so that O is rescaled a few times per range and not once per tile
+        bf16x8 pf[NC];
+        auto visible = [&](int cb, int key) -> bool { return key < base || (key < total && ((see[cb] >> (key - base)) & 1)); };
+#pragma unroll
+        for (int cb = 0; cb < NC; ++cb) {
+            float p[2][4], mx = -INFINITY;
+#pragma unroll
+            for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = st[cb][kf][r] * (FMT == KV_BF16 ? kmul : ksv[kf][r]);
+                    if (edge && !visible(cb, k0 + kf * 16 + g * 4 + r)) x = -INFINITY;
+                    p[kf][r] = x;
+                    mx = fmaxf(mx, x);
+                }
+            mx = group_max(mx);
+            if (__any(mx > m_run[cb] + 8.f)) {
+                const float m_new = mx > m_run[cb] + 8.f ? mx : m_run[cb];
+                const float alpha = m_run[cb] == m_new ? 1.f : __builtin_amdgcn_exp2f(m_run[cb] - m_new);
+                m_run[cb] = m_new;
+                l_run[cb] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DF; ++d) oacc[cb][d] *= alpha;
+            }
+            const float m = m_run[cb] == -INFINITY ? 0.f : m_run[cb];     // nothing seen yet: every weight is 0
+            float sum = 0.f;
+#pragma unroll
+            for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[kf][r] = __builtin_amdgcn_exp2f(p[kf][r] - m);
+                    sum += p[kf][r];
+                    if (FMT != KV_BF16) {
+                        p[kf][r] *= vsv[kf][r];
+                        if (edge && !visible(cb, k0 + kf * 16 + g * 4 + r)) p[kf][r] = 0.f;    // (the scale of a hidden row may be NaN)
+                    }
+                }
+            l_run[cb] += sum;
+            pf[cb] = __builtin_bit_cast(bf16x8, make_uint4(pack_bf2(p[0][0], p[0][1]), pack_bf2(p[0][2], p[0][3]), pack_bf2(p[1][0], p[1][1]), pack_bf2(p[1][2], p[1][3])));
+        }
+        // ---- O^T += V^T . P^T; slot j of lane group g is key (j >> 2) * 16 + 4 g + (j & 3)
+        if (FMT == KV_BF16 && __any(odd_v)) {             // rare: a product with a hidden NaN or infinity would be NaN; add visible keys one by one
+            for (int key = 0; key < TK; ++key)
+#pragma unroll
+                for (int cb = 0; cb < NC; ++cb) {
+                    // the key's weight sits in the lanes of group (key & 15) >> 2, pair (key >> 4, (key & 3) >> 1) of the packed operand
+                    const uint4 pk = __builtin_bit_cast(uint4, pf[cb]);
+                    const uint32_t mine = key < 16 ? ((key & 2) ? pk.y : pk.x) : ((key & 2) ? pk.w : pk.z);
+                    const uint32_t pair = (uint32_t)__shfl((int)mine, ((key & 15) >> 2) * 16 + l15, 64);
+                    const float w = (key & 1) ? bf_hi(pair) : bf_lo(pair);
+                    const bool on = visible(cb, k0 + key);
+#pragma unroll
+                    for (int df = 0; df < DF; ++df)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int d = df * 16 + g * 4 + r;
+                            const float x = bf2f(*(const bf16_t*)(vimg + key * T::RB + (((d >> 3) ^ T::swz(key)) * 16) + (d & 7) * 2));
+                            if (on) oacc[cb][df][r] += w * x;
+                        }
+                }
+            continue;
+        }
+#pragma unroll
+        for (int df = 0; df < DF; ++df) {
+            bf16x8 vf;
+            if (FMT == KV_BF16) {
+                const int chunk = df * 2 + ((l15 & 3) >> 1), sub = (l15 & 1) * 8, r0 = 4 * g + (l15 >> 2), r1 = r0 + 16;
+                typedef __attribute__((ext_vector_type(4))) short s16x4;
+                typedef __attribute__((ext_vector_type(8))) short s16x8;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vimg + r0 * T::RB + ((chunk ^ T::swz(r0)) * 16) + sub));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vimg + r1 * T::RB + ((chunk ^ T::swz(r1)) * 16) + sub));
+                const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                vf = __builtin_bit_cast(bf16x8, both);
+            } else {
+                // (lane i of a 16-lane group supplies 8 bytes of row i >> 1, columns 8 (i & 1) ..; it receives column i of the 8 rows)
+                typedef __attribute__((ext_vector_type(2))) int i32x2;
+                const int r = l15 >> 1, row = (r >> 2) * 16 + 4 * g + (r & 3);
+                const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(vimg + row * T::RB + ((df ^ T::swz(row)) * 16) + (l15 & 1) * 8));
+                vf = codes_to_bf16<FMT>(make_uint2((uint32_t)x[0], (uint32_t)x[1]));
+            }
+#pragma unroll
+            for (int cb = 0; cb < NC; ++cb) oacc[cb][df] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[cb], oacc[cb][df], 0, 0, 0);
+        }
+    }
+
+    // ---- join the waves, one block of 16 columns at a time: [wave][column][D + 4 floats], [wave][column] (m, l)
+    float* jo = (float*)smem;
+    float2* jm = (float2*)(smem + 4 * 16 * (D + 4) * 4);
+    constexpr int PER = D / 16;                           // floats per thread
+    const int jc = tid >> 4, jd = (tid & 15) * PER;
+#pragma unroll
+    for (int cb = 0; cb < NC; ++cb) {
+        __syncthreads();
+        float l = l_run[cb];
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+#pragma unroll
+        for (int df = 0; df < DF; ++df)
+            *(float4*)(jo + (wave * 16 + l15) * (D + 4) + df * 16 + g * 4) = make_float4(oacc[cb][df][0], oacc[cb][df][1], oacc[cb][df][2], oacc[cb][df][3]);
+        if (g == 0) jm[wave * 16 + l15] = make_float2(m_run[cb], l);
+        __syncthreads();
+        int row, head, node;
+        if (!col_info(c0 + cb * 16 + jc, row, head, node)) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * 16 + jc].x);
+        float L = 0.f, O[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) O[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 ml = jm[w * 16 + jc];
+            const float f = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+            L += ml.y * f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) O[i] += jo[(w * 16 + jc) * (D + 4) + jd + i] * f;
+        }
+        const long col = ((long)row * A.N + node) * A.Hq + head;
+        float* ro = A.rec_o + ((long)slot * ncol_all + col) * D + jd;
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) *(float4*)(ro + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
+        if ((tid & 15) == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
+    }
+}
+
+template <int FMT, int D, int NCA, int NCB>
+__global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs A) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int rep = A.Hq / A.Hkv;
+    const bool role_a = (int)blockIdx.x < A.na;
+    // column blocks of one (keys, range) go to one XCD (workgroups are dealt to the 8 XCDs in turn), next to each other: its L2 serves all but the first
+    const int idx = role_a ? blockIdx.x : blockIdx.x - A.na, cbs = role_a ? A.cba : A.cbb;
+    const int cb = (idx >> 3) % cbs, job = ((idx >> 3) / cbs) * 8 + (idx & 7);
+    if (role_a) {
+        const int sp = job % A.sa, hk = (job / A.sa) % A.Hkv, pr = job / (A.sa * A.Hkv);
+        if (pr >= A.n_prompts) return;
+        const int r0 = A.row0 ? min(max(A.row0[pr], 0), A.B) : min(pr * A.rows, A.B);
+        const int r1 = A.row0 ? min(max(A.row0[pr + 1], r0), A.B) : min((pr + 1) * A.rows, A.B);
+        const int nrow = min(r1 - r0, A.rows), ncol = nrow * A.N * rep, c0 = cb * 16 * NCA;
+        if (c0 >= ncol) return;
+        const int total = min(max(A.prompt_len[pr], 0), A.prompt.cap);
+        const int nt = (total + TK - 1) / TK, per = (nt + A.sa - 1) / A.sa, t0 = sp * per, t1 = min(nt, t0 + per);
+        const long kv = ((long)pr * A.prompt.s_seq + (long)hk * A.prompt.s_head) * kv_size<FMT>(), ks = (long)pr * A.prompt.c_seq + (long)hk * A.prompt.c_head;
+        const int per_row = A.N * rep;
+        attend<FMT, D, NCA>(A, smem, A.prompt.k + kv, A.prompt.v + kv, A.prompt.ks + ks, A.prompt.vs + ks, A.prompt.s_pos, A.prompt.c_pos, total, total, t0,
+                            t1, c0, sp, [&](int c, int& row, int& head, int& node) -> bool {
+                                const int r = c / per_row, x = c - r * per_row;
+                                row = r0 + r; node = x / rep; head = hk * rep + x - node * rep;
+                                return c < ncol;
+                            });
+    } else {
+        const int sp = job % A.sb, hk = (job / A.sb) % A.Hkv, b = job / (A.sb * A.Hkv);
+        if (b >= A.B) return;
+        const int ncol = A.N * rep, c0 = cb * 16 * NCB;
+        if (c0 >= ncol) return;
+        const int base = min(max(A.tail_len[(long)b * A.len_stride], 0), A.tail.cap), total = min(base + A.N, A.tail.cap);
+        const int nt = (total + TK - 1) / TK, per = (nt + A.sb - 1) / A.sb, t0 = sp * per, t1 = min(nt, t0 + per);
+        const long kv = ((long)b * A.tail.s_seq + (long)hk * A.tail.s_head) * kv_size<FMT>(), ks = (long)b * A.tail.c_seq + (long)hk * A.tail.c_head;
+        attend<FMT, D, NCB>(A, smem, A.tail.k + kv, A.tail.v + kv, A.tail.ks + ks, A.tail.vs + ks, A.tail.s_pos, A.tail.c_pos, total, base, t0, t1, c0,
+                            A.sa + sp, [&](int c, int& row, int& head, int& node) -> bool {
+                                row = b; node = c / rep; head = hk * rep + c - node * rep;
+                                return c < ncol;
+                            });
+    }
+}
+
+// o = the softmax-weighted join of a column's records; D / 4 lanes per column.  A sequence that no prompt owns has no prompt records.
+template <int D>
+__global__ __launch_bounds__(256) void attn_cache_join_kernel(const AttnCacheArgs A) {
+    constexpr int LPC = D / 4;
+    const long ncol = (long)A.B * A.N * A.Hq;
+    const long col = (long)blockIdx.x * (256 / LPC) + threadIdx.x / LPC;
+    if (col >= ncol) return;
+    const int d = (threadIdx.x % LPC) * 4, b = (int)(col / ((long)A.N * A.Hq));
+    int first = 0;
+    if (A.sa) {
+        const int lo = A.row0 ? A.row0[0] : 0, hi = A.row0 ? A.row0[A.n_prompts] : A.n_prompts * A.rows;
+        if (b < lo || b >= hi) first = A.sa;
+    }
+    const int ns = A.sa + A.sb;
+    float M = -INFINITY;
+#pragma unroll 4
+    for (int s = first; s < ns; ++s) M = fmaxf(M, A.rec_ml[s * ncol + col].x);
+    float L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = first; s < ns; ++s) {
+        const float2 ml = A.rec_ml[s * ncol + col];
+        const float4 x = *(const float4*)(A.rec_o + (s * ncol + col) * D + d);
+        const float f = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+        L += ml.y * f;
+        O[0] += x.x * f; O[1] += x.y * f; O[2] += x.z * f; O[3] += x.w * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *(uint2*)(A.o + col * D + d) = make_uint2(pack_bf2(O[0] * inv, O[1] * inv), pack_bf2(O[2] * inv, O[3] * inv));
+}
+
+struct AttnPlan {
+    int nca, ncb, cba, cbb, sa, sb;
+    long cols;
+};
+
+// Column blocks: as wide as the columns need, up to 64 (a wave's fp32 O of 64 x 128 is 128 registers).  Key ranges: the launch's keys x column
+// blocks spread over 512 workgroups (two per CU, all resident), at least 256 keys (two tiles per wave) each; the capacities stand for the lengths,
+// which only the device knows.
+AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
+    const spacer_kv_cache* c = prompt ? prompt : tail;
+    const int rep = Hq / c->kv_heads;
+    const long ca = prompt ? (long)rows * N * rep : 0, cb = tail ? (long)N * rep : 0;
+    AttnPlan p;
+    const long most = ca > cb ? ca : cb;
+    if (most <= 16) p.nca = p.ncb = 1;
+    else if (cb <= 16) { p.nca = 4; p.ncb = 1; }
+    else if (most <= 32) p.nca = p.ncb = 2;
+    else p.nca = p.ncb = 4;
+    p.cba = prompt ? cdiv(ca, 16 * p.nca) : 0;
+    p.cbb = tail ? cdiv(cb, 16 * p.ncb) : 0;
+    const double ja = prompt ? (double)prompt->n_seq * c->kv_heads * p.cba : 0, jb = tail ? (double)B * c->kv_heads * p.cbb : 0;
+    double keys = (prompt ? ja * prompt->capacity : 0) + (tail ? jb * tail->capacity : 0);
+    keys /= 512;
+    const long range = keys < 256 ? 256 : keys > 1e9 ? 1000000000L : (long)keys + 1;
+    p.sa = prompt ? cdiv(prompt->capacity, range) : 0;
+    p.sb = tail ? cdiv(tail->capacity, range) : 0;
+    p.cols = (long)B * N * Hq;
+    return p;
+}
+
+}  // namespace
+
+static int check_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
+    SP_REQUIRE(prompt || tail, SPACER_EINVAL, "attn_cache: no cache");
+    if (prompt)
+        if (int rc = spacer_check_kv_cache(prompt, "attn_cache")) return rc;
+    if (tail)
+        if (int rc = spacer_check_kv_cache(tail, "attn_cache")) return rc;
+    SP_REQUIRE(!prompt || !tail || (prompt->format == tail->format && prompt->kv_heads == tail->kv_heads && prompt->head_dim == tail->head_dim),
+               SPACER_EINVAL, "attn_cache: prompt and tail caches differ in format, kv_heads or head_dim");
+    const spacer_kv_cache* c = prompt ? prompt : tail;
+    SP_REQUIRE(B >= 0 && N >= 1 && N <= 64, SPACER_EINVAL, "attn_cache: %d sequences, %d nodes (1 .. 64)", B, N);
+    SP_REQUIRE(Hq > 0 && Hq % c->kv_heads == 0, SPACER_EINVAL, "attn_cache: %d query heads over %d kv heads", Hq, c->kv_heads);
+    SP_REQUIRE(!prompt || rows > 0, SPACER_EINVAL, "attn_cache: rows = %d per prompt", rows);
+    SP_REQUIRE(!tail || tail->n_seq == B, SPACER_EINVAL, "attn_cache: tail cache of %d sequences, %d queries", tail ? tail->n_seq : 0, B);
+    SP_REQUIRE((long)B * N * Hq <= 0x3fffffffL && (long)rows * N * Hq <= 0x3fffffffL, SPACER_EINVAL, "attn_cache: too many queries");
+    return SPACER_OK;
+}
+
+extern "C" long spacer_attn_cache_workspace_bytes(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
+    if (check_attn(prompt, tail, rows, B, N, Hq)) return -1;
+    const AttnPlan p = plan_attn(prompt, tail, rows, B, N, Hq);
+    const int D = prompt ? prompt->head_dim : tail->head_dim;
+    return (p.sa + p.sb) * p.cols * (D + 2) * 4L;
+}
+
+extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache* prompt, const int* prompt_len, const int* row0, int rows,
+                                 const spacer_kv_cache* tail, const int* tail_len, int len_per_seq, const int64_t* tree, int tree_per_seq, void* o,
+                                 int B, int N, int Hq, float scale, void* workspace, long workspace_bytes, spacer_stream_t stream) {
+    if (int rc = check_attn(prompt, tail, rows, B, N, Hq)) return rc;
+    if (B == 0) return SPACER_OK;
+    const spacer_kv_cache* c = prompt ? prompt : tail;
+    const int D = c->head_dim, Hkv = c->kv_heads;
+    SP_REQUIRE(q && o && (((uintptr_t)q | (uintptr_t)o) & 15) == 0 && q_ld % 8 == 0, SPACER_EINVAL, "attn_cache: q and o rows must start at multiples of 16 bytes");
+    SP_REQUIRE(!prompt || prompt_len, SPACER_EINVAL, "attn_cache: prompt_len required");
+    SP_REQUIRE(!prompt || row0 || (long)prompt->n_seq * rows == B, SPACER_EINVAL, "attn_cache: %d prompts x %d rows, %d sequences", prompt ? prompt->n_seq : 0, rows, B);
+    SP_REQUIRE(!tail || tail_len, SPACER_EINVAL, "attn_cache: tail_len required");
+    const AttnPlan p = plan_attn(prompt, tail, rows, B, N, Hq);
+    const long need = (p.sa + p.sb) * p.cols * (D + 2) * 4L;
+    SP_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, SPACER_ENOMEM, "attn_cache: workspace of %ld bytes, %ld needed",
+               workspace ? workspace_bytes : 0L, need);
+    AttnCacheArgs A = {};
+    A.q = (const bf16_t*)q; A.q_ld = q_ld;
+    if (prompt) { A.prompt = spacer_kv_view(prompt); A.n_prompts = prompt->n_seq; }
+    if (tail) A.tail = spacer_kv_view(tail);
+    A.prompt_len = prompt_len; A.tail_len = tail_len; A.row0 = row0; A.tree = tree;
+    A.len_stride = len_per_seq ? 1 : 0; A.tree_stride = tree_per_seq ? N : 0;
+    A.rows = rows; A.B = B; A.N = N; A.Hq = Hq; A.Hkv = Hkv;
+    A.sa = p.sa; A.sb = p.sb; A.cba = p.cba; A.cbb = p.cbb;
+    A.scale = scale;
+    A.rec_o = (float*)workspace;
+    A.rec_ml = (float2*)(A.rec_o + (p.sa + p.sb) * p.cols * D);
+    A.o = (bf16_t*)o;
+    const long ja = prompt ? (long)prompt->n_seq * Hkv * p.sa : 0, jb = tail ? (long)B * Hkv * p.sb : 0;
+    const long na = (ja + 7) / 8 * 8 * p.cba, nb = (jb + 7) / 8 * 8 * p.cbb;
+    SP_REQUIRE(na + nb <= 0x7fffffffL, SPACER_EINVAL, "attn_cache: too many workgroups");
+    A.na = (int)na;
+    hipStream_t s = (hipStream_t)stream;
+#define LAUNCH(F, DD, NA, NB)                                                                                                                       \
+    hipLaunchKernelGGL((attn_cache_kernel<F, DD, NA, NB>), dim3((unsigned)(na + nb)), dim3(256), lds_bytes(kv_size<F>(), DD, NA > NB ? NA : NB), s, A)
+#define CALL(F, DD)                                                                                                                                 \
+    do {                                                                                                                                            \
+        if (p.nca == 1) LAUNCH(F, DD, 1, 1);                                                                                                        \
+        else if (p.nca == 2) LAUNCH(F, DD, 2, 2);                                                                                                   \
+        else if (p.ncb == 1) LAUNCH(F, DD, 4, 1);                                                                                                   \
+        else LAUNCH(F, DD, 4, 4);                                                                                                                   \
+    } while (0)
+    KV_DISPATCH(c, CALL);
+#undef CALL
+#undef LAUNCH
+    if (D == 128) hipLaunchKernelGGL(attn_cache_join_kernel<128>, dim3(cdiv(p.cols, 8)), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL(attn_cache_join_kernel<64>, dim3(cdiv(p.cols, 16)), dim3(256), 0, s, A);
+    SP_CHECK_LAUNCH();
+    return SPACER_OK;
+}

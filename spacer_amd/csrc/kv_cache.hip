@@ -1,0 +1,286 @@
+// Writers and reader of the rollout's key/value cache (bf16, e4m3 or int8 rows; layout and row arithmetic: kv_cache.h).
+//
+//   kv_write    one source row per (sequence, position) slot: a prompt batch's K / V columns of the packed q|k|v rows -> the cache
+//   kv_append   the N newest tokens of every sequence -> positions len .. len + N - 1 of its own cache
+//   kv_read     the cache's values as bf16 or fp32 rows [sequence, position, kv head, D]
+//   decode_qkv_finish_cache   the decode step's form of kv_append: split-K sums + bias + rotary -> q, and K / V into the cache
+//
+// All four move each byte once and are bound by memory: D / 8 lanes hold a row (16-byte loads), K and V of a row are in flight together.
+#include "kv_cache.h"
+
+namespace {
+
+template <int FMT, int D>
+__device__ __forceinline__ void store_row(char* dst, float* scale, const uint4 x, int lane_in_row) {
+    constexpr int LPR = D / 8;
+    if (FMT == KV_BF16) {
+        *(uint4*)(dst + lane_in_row * 16) = x;
+        return;
+    }
+    uint32_t a = max(max(amax2(x.x), amax2(x.y)), max(amax2(x.z), amax2(x.w)));
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
+    const RowScale r = row_scale<FMT>(a);
+    const uint32_t lo = code2<FMT>(x.x, r) | (code2<FMT>(x.y, r) << 16), hi = code2<FMT>(x.z, r) | (code2<FMT>(x.w, r) << 16);
+    *(uint2*)(dst + lane_in_row * 8) = make_uint2(lo, hi);
+    if (lane_in_row == 0) *scale = r.scale;
+}
+
+// APPEND == false: row (slot, head) takes source row rows[slot] (below 0, or >= n_src: the slot stays as it is)
+// APPEND == true : row (b N + i, head) goes to position len[b] + i of sequence b (outside the cache: dropped)
+template <int FMT, int D, bool APPEND>
+__global__ __launch_bounds__(256) void kv_store_kernel(const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, long ld, int n_src,
+                                                       const int* __restrict__ rows, const int* __restrict__ len, int len_stride, int N,
+                                                       KvView c, int Hkv, long total) {
+    constexpr int LPR = D / 8, RPW = 64 / LPR;       // lanes per row, rows per wave
+    const int lane = threadIdx.x & 63, lr = lane % LPR;
+    const long nw = (long)gridDim.x * 4;
+    // (row ids of one wave are consecutive: the heads of a token lie side by side in the source)
+    for (long r0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW; r0 < total; r0 += nw * RPW) {
+        const long rid = r0 + lane / LPR;
+        long src = -1;
+        int seq = 0, pos = 0, h = 0;
+        if (rid < total) {
+            h = (int)(rid % Hkv);
+            const long slot = rid / Hkv;
+            if (APPEND) {
+                seq = (int)(slot / N);
+                const long p = (long)len[(long)seq * len_stride] + slot % N;
+                src = (p >= 0 && p < c.cap) ? slot : -1;
+                pos = (int)p;
+            } else {
+                seq = (int)(slot / c.cap);
+                pos = (int)(slot % c.cap);
+                src = rows[slot];
+                if (src >= n_src) src = -1;
+            }
+        }
+        const bool live = src >= 0;
+        uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
+        if (live) {
+            xk = *(const uint4*)(k + src * ld + h * D + lr * 8);
+            xv = *(const uint4*)(v + src * ld + h * D + lr * 8);
+        }
+        if (!live) continue;                         // (whole rows drop out: the lanes of a row stay together)
+        const long at = (seq * c.s_seq + h * c.s_head + pos * c.s_pos) * kv_size<FMT>();
+        const long sat = seq * c.c_seq + h * c.c_head + pos * c.c_pos;
+        store_row<FMT, D>(c.k + at, c.ks + sat, xk, lr);
+        store_row<FMT, D>(c.v + at, c.vs + sat, xv, lr);
+    }
+}
+
+template <int FMT>
+__device__ __forceinline__ void values8(const char* p, float s, float (&f)[8]) {
+    if (FMT == KV_BF16) {
+        const uint4 x = *(const uint4*)p;
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); }
+        return;
+    }
+    const uint2 x = *(const uint2*)p;
+    const uint32_t w[2] = {x.x, x.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (FMT == KV_E4M3) {
+            const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+            f[4 * i] = a[0]; f[4 * i + 1] = a[1]; f[4 * i + 2] = b[0]; f[4 * i + 3] = b[1];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[4 * i + j] = (float)(int8_t)((w[i] >> (8 * j)) & 0xffu);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= s;
+}
+
+template <int FMT, int D, bool F32>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvView c, const int* __restrict__ len, void* __restrict__ ko, void* __restrict__ vo,
+                                                      int Hkv, long total) {
+    constexpr int LPR = D / 8, RPW = 64 / LPR;
+    const int lane = threadIdx.x & 63, lr = lane % LPR;
+    const long nw = (long)gridDim.x * 4;
+    for (long r0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW; r0 < total; r0 += nw * RPW) {
+        const long rid = r0 + lane / LPR;
+        if (rid >= total) continue;
+        const int h = (int)(rid % Hkv);
+        const long slot = rid / Hkv;
+        const int seq = (int)(slot / c.cap), pos = (int)(slot % c.cap);
+        float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (!len || pos < len[seq]) {
+            const long at = (seq * c.s_seq + h * c.s_head + pos * c.s_pos + lr * 8) * kv_size<FMT>();
+            const long sat = seq * c.c_seq + h * c.c_head + pos * c.c_pos;
+            const float sk = FMT == KV_BF16 ? 1.f : c.ks[sat], sv = FMT == KV_BF16 ? 1.f : c.vs[sat];
+            values8<FMT>(c.k + at, sk, a);
+            values8<FMT>(c.v + at, sv, b);
+        }
+        const long o = rid * D + lr * 8;
+        if (F32) {
+            float *kp = (float*)ko + o, *vp = (float*)vo + o;
+            *(float4*)kp = make_float4(a[0], a[1], a[2], a[3]); *(float4*)(kp + 4) = make_float4(a[4], a[5], a[6], a[7]);
+            *(float4*)vp = make_float4(b[0], b[1], b[2], b[3]); *(float4*)(vp + 4) = make_float4(b[4], b[5], b[6], b[7]);
+        } else {
+            *(uint4*)((bf16_t*)ko + o) = make_uint4(pack_bf2(a[0], a[1]), pack_bf2(a[2], a[3]), pack_bf2(a[4], a[5]), pack_bf2(a[6], a[7]));
+            *(uint4*)((bf16_t*)vo + o) = make_uint4(pack_bf2(b[0], b[1]), pack_bf2(b[2], b[3]), pack_bf2(b[4], b[5]), pack_bf2(b[6], b[7]));
+        }
+    }
+}
+
+// One wave per (sequence, head) of the step's q|k|v sums; lane j < D / 2 holds the rotary pair (j, j + D / 2).  K and V are rounded to
+// bf16 first and quantised from there, so that the cache holds what kv_append makes of the same bf16 rows.
+template <int FMT>
+__global__ __launch_bounds__(256) void decode_qkv_finish_cache_kernel(float* __restrict__ acc, const bf16_t* __restrict__ bias,
+                                                                      const float* __restrict__ cs, const float* __restrict__ sn,
+                                                                      bf16_t* __restrict__ q_out, KvView c, const int* __restrict__ tail_len,
+                                                                      int len_stride, int B, int Hq, int Hkv, int D,
+                                                                      const float* __restrict__ rowss, float* __restrict__ rowss_zero,
+                                                                      int norm_cols, float eps) {
+    const int lane = threadIdx.x & 63, half = D / 2, heads = Hq + 2 * Hkv;
+    if (rowss_zero && blockIdx.x == 0 && threadIdx.x < B) rowss_zero[threadIdx.x] = 0.f;
+    const int wid = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (wid >= B * heads) return;
+    const int b = wid / heads, hh = wid % heads;
+    const int j = min(lane, half - 1);
+    const bool on = lane < half;
+    float* a = acc + (long)wid * D;
+    // every load before the first use: absent operands read a valid dummy address and are masked
+    const bf16_t* bias_p = bias ? bias + (long)hh * D : (const bf16_t*)cs;
+    const float bias_on = bias ? 1.f : 0.f;
+    const int pos = tail_len[(long)b * len_stride];
+    const float rsum = rowss ? rowss[b] : 0.f;
+    const float a1 = a[j], a2 = a[j + half];
+    const bf16_t b1 = bias_p[bias ? j : 0], b2 = bias_p[bias ? j + half : 0];
+    const float c1 = cs[(long)b * D + j], s1 = sn[(long)b * D + j], c2 = cs[(long)b * D + j + half], s2 = sn[(long)b * D + j + half];
+    const float rs = rowss ? rsqrtf(rsum / (float)norm_cols + eps) : 1.f;
+    float x1 = a1 * rs + bias_on * bf2f(b1), x2 = a2 * rs + bias_on * bf2f(b2);
+    if (on) { a[j] = 0.f; a[j + half] = 0.f; }
+    if (hh < Hq + Hkv) {
+        const float r1 = x1 * c1 - x2 * s1, r2 = x2 * c2 + x1 * s2;
+        x1 = r1; x2 = r2;
+    }
+    const uint32_t w = pack_bf2(x1, x2);
+    if (hh < Hq) {
+        bf16_t* dst = q_out + ((long)b * Hq + hh) * D;
+        if (on) { dst[j] = (bf16_t)(w & 0xffffu); dst[j + half] = (bf16_t)(w >> 16); }
+        return;
+    }
+    if (pos < 0 || pos >= c.cap) return;
+    const bool is_k = hh < Hq + Hkv;
+    const int h = hh - Hq - (is_k ? 0 : Hkv);
+    char* dst = (is_k ? c.k : c.v) + (b * c.s_seq + h * c.s_head + pos * c.s_pos) * kv_size<FMT>();
+    if (FMT == KV_BF16) {
+        if (on) { ((bf16_t*)dst)[j] = (bf16_t)(w & 0xffffu); ((bf16_t*)dst)[j + half] = (bf16_t)(w >> 16); }
+        return;
+    }
+    uint32_t m = amax2(w);                           // (lanes past half repeat the last pair: the maximum is the same)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    const RowScale r = row_scale<FMT>(m);
+    const uint32_t q = code2<FMT>(w, r);
+    if (on) { dst[j] = (char)(q & 0xffu); dst[j + half] = (char)(q >> 8); }
+    if (lane == 0) (is_k ? c.ks : c.vs)[b * c.c_seq + h * c.c_head + pos * c.c_pos] = r.scale;
+}
+
+}  // namespace
+
+// ---- host: one check of a cache for every entry that takes one
+int spacer_check_kv_cache(const spacer_kv_cache* c, const char* who) {
+    SP_REQUIRE(c, SPACER_EINVAL, "%s: no cache", who);
+    SP_REQUIRE(c->struct_bytes == (int)sizeof(spacer_kv_cache), SPACER_EINVAL, "%s: spacer_kv_cache: struct_bytes = %d but this library's has %d bytes",
+               who, c->struct_bytes, (int)sizeof(spacer_kv_cache));
+    SP_REQUIRE(c->format == KV_BF16 || c->format == KV_E4M3 || c->format == KV_INT8, SPACER_EINVAL, "%s: cache format %d unknown", who, c->format);
+    SP_REQUIRE(c->head_dim == 64 || c->head_dim == 128, SPACER_EINVAL, "%s: head_dim %d unsupported (64, 128)", who, c->head_dim);
+    SP_REQUIRE(c->n_seq > 0 && c->capacity > 0 && c->kv_heads > 0, SPACER_EINVAL, "%s: empty cache (%d sequences, %d positions, %d heads)", who,
+               c->n_seq, c->capacity, c->kv_heads);
+    SP_REQUIRE(c->k && c->v, SPACER_EINVAL, "%s: cache without k or v", who);
+    const long size = c->format == KV_BF16 ? 2 : 1;
+    SP_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0 && ((c->stride_seq | c->stride_head | c->stride_pos) * size) % 16 == 0, SPACER_EINVAL,
+               "%s: cache rows must start at multiples of 16 bytes", who);
+    SP_REQUIRE(c->format == KV_BF16 || (c->k_scale && c->v_scale), SPACER_EINVAL, "%s: 8-bit cache without scales", who);
+    return SPACER_OK;
+}
+
+KvView spacer_kv_view(const spacer_kv_cache* c) {
+    return KvView{(char*)c->k, (char*)c->v, c->k_scale, c->v_scale, c->stride_seq, c->stride_head, c->stride_pos, c->scale_stride_seq,
+                  c->scale_stride_head, c->scale_stride_pos, c->n_seq, c->capacity};
+}
+
+// workgroups of a row pass: 4 waves each, enough to cover the rows, at most 16 per CU (the loop strides over the rest)
+static int row_grid(long total, int D) { return (int)min(cdiv(total, 4 * (512 / D)), 256 * 16); }
+
+static int check_source(const void* k, const void* v, long ld, const char* who) {
+    SP_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ld % 8 == 0, SPACER_EINVAL, "%s: source rows must start at multiples of 16 bytes", who);
+    return SPACER_OK;
+}
+
+extern "C" int spacer_kv_write(const spacer_kv_cache* c, const void* k, const void* v, long ld, int n_src, const int* rows, spacer_stream_t stream) {
+    if (int rc = spacer_check_kv_cache(c, "kv_write")) return rc;
+    SP_REQUIRE(n_src >= 0 && rows, SPACER_EINVAL, "kv_write: rows required, n_src >= 0");
+    if (n_src == 0) return SPACER_OK;
+    if (int rc = check_source(k, v, ld, "kv_write")) return rc;
+    const long total = (long)c->n_seq * c->capacity * c->kv_heads;
+#define CALL(F, D)                                                                                                                                   \
+    hipLaunchKernelGGL((kv_store_kernel<F, D, false>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
+                       ld, n_src, rows, (const int*)nullptr, 0, 1, spacer_kv_view(c), c->kv_heads, total)
+    KV_DISPATCH(c, CALL);
+#undef CALL
+    SP_CHECK_LAUNCH();
+    return SPACER_OK;
+}
+
+extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const void* v, long ld, int N, const int* len, int len_per_seq,
+                                spacer_stream_t stream) {
+    if (int rc = spacer_check_kv_cache(c, "kv_append")) return rc;
+    SP_REQUIRE(N >= 0 && len, SPACER_EINVAL, "kv_append: lengths required, N >= 0");
+    if (N == 0) return SPACER_OK;
+    if (int rc = check_source(k, v, ld, "kv_append")) return rc;
+    SP_REQUIRE((long)c->n_seq * N <= 0x7fffffffL, SPACER_EINVAL, "kv_append: %d sequences x %d tokens are too many", c->n_seq, N);
+    const long total = (long)c->n_seq * N * c->kv_heads;
+#define CALL(F, D)                                                                                                                                  \
+    hipLaunchKernelGGL((kv_store_kernel<F, D, true>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
+                       ld, c->n_seq * N, (const int*)nullptr, len, len_per_seq ? 1 : 0, N, spacer_kv_view(c), c->kv_heads, total)
+    KV_DISPATCH(c, CALL);
+#undef CALL
+    SP_CHECK_LAUNCH();
+    return SPACER_OK;
+}
+
+extern "C" int spacer_kv_read(const spacer_kv_cache* c, const int* len, void* k_out, void* v_out, int out_f32, spacer_stream_t stream) {
+    if (int rc = spacer_check_kv_cache(c, "kv_read")) return rc;
+    SP_REQUIRE(k_out && v_out && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, SPACER_EINVAL, "kv_read: outputs must be 16-byte aligned");
+    const long total = (long)c->n_seq * c->capacity * c->kv_heads;
+#define CALL(F, D)                                                                                                                                   \
+    do {                                                                                                                                             \
+        if (out_f32)                                                                                                                                 \
+            hipLaunchKernelGGL((kv_read_kernel<F, D, true>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, spacer_kv_view(c), len, k_out, \
+                               v_out, c->kv_heads, total);                                                                                           \
+        else                                                                                                                                         \
+            hipLaunchKernelGGL((kv_read_kernel<F, D, false>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, spacer_kv_view(c), len, k_out, \
+                               v_out, c->kv_heads, total);                                                                                           \
+    } while (0)
+    KV_DISPATCH(c, CALL);
+#undef CALL
+    SP_CHECK_LAUNCH();
+    return SPACER_OK;
+}
+
+extern "C" int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, const float* cos_t, const float* sin_t, void* q_out,
+                                              const spacer_kv_cache* c, const int* tail_len, int len_per_seq, const float* rowss, float* rowss_zero,
+                                              int norm_cols, float eps, int Hq, spacer_stream_t stream) {
+    if (int rc = spacer_check_kv_cache(c, "decode_qkv_finish_cache")) return rc;
+    const int B = c->n_seq, heads = Hq + 2 * c->kv_heads;
+    SP_REQUIRE(acc32 && cos_t && sin_t && q_out && tail_len, SPACER_EINVAL, "decode_qkv_finish_cache: missing operand");
+    SP_REQUIRE(Hq > 0, SPACER_EINVAL, "decode_qkv_finish_cache: Hq = %d", Hq);
+    SP_REQUIRE(!rowss || norm_cols > 0, SPACER_EINVAL, "decode_qkv_finish_cache: norm_cols = %d", norm_cols);
+    SP_REQUIRE(!rowss_zero || B <= 256, SPACER_EINVAL, "decode_qkv_finish_cache: at most 256 rows with rowss_zero, got %d", B);
+    const dim3 grid(cdiv((long)B * heads, 4)), block(256);
+#define CALL(F)                                                                                                                                     \
+    hipLaunchKernelGGL((decode_qkv_finish_cache_kernel<F>), grid, block, 0, (hipStream_t)stream, acc32, (const bf16_t*)bias, cos_t, sin_t, (bf16_t*)q_out, \
+                       spacer_kv_view(c), tail_len, len_per_seq ? 1 : 0, B, Hq, c->kv_heads, c->head_dim, rowss, rowss_zero, norm_cols, eps)
+    if (c->format == KV_BF16) CALL(KV_BF16);
+    else if (c->format == KV_E4M3) CALL(KV_E4M3);
+    else CALL(KV_INT8);
+#undef CALL
+    SP_CHECK_LAUNCH();
+    return SPACER_OK;
+}

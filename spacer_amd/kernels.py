@@ -455,6 +455,270 @@ def attn_decode_shared_rows(q, prefix_k, prefix_v, prefix_len, prompt_of, row0, 
     return out
 
 
+# ----------------------------------------------------------------------------------------- key/value cache in 16 or 8 bits
+def _require(ok, what: str) -> None:
+    if not ok:
+        raise SpacerError(what)
+
+
+def _on_current_device(*tensors) -> None:
+    """The launch goes to the current device's current stream: a tensor of another device is refused, not read across the link."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise SpacerError(f"tensor on {t.device}, but the current device is cuda:{cur} (use torch.cuda.device)")
+
+
+def _i32(t, n, what: str) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
+        raise SpacerError(f"{what}: expected {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
+
+
+_KV_FORMATS = {torch.bfloat16: _lib.SPACER_KV_BF16, torch.float8_e4m3fn: _lib.SPACER_KV_E4M3, torch.int8: _lib.SPACER_KV_INT8}
+KV_DTYPES = {"bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+class KVCache:
+    """Keys and values of ``n_seq`` sequences x ``capacity`` positions x ``kv_heads`` rows of ``head_dim`` (64 or 128) numbers: k, v
+    [n_seq, kv_heads, capacity, head_dim] in bf16, float8_e4m3fn or int8, the last dimension contiguous, any strides otherwise (k and v
+    the same; a transposed view of [n_seq, capacity, kv_heads, head_dim] works).  8-bit rows carry one fp32 scale each, k_scale / v_scale
+    [n_seq, kv_heads, capacity], and stand for code * scale:
+        float8_e4m3fn   scale = the smallest power of two >= 2^-126 with max|row| / scale <= 448
+        int8            scale = max|row| / 127, codes -127 .. 127, ties of x / scale to even
+    A row that holds a NaN or an infinity gets scale NaN.  The object only describes the tensors (and keeps them alive)."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "kv_heads", "capacity", "head_dim", "dtype", "device", "_c", "_ref")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        _require(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and k.device == v.device,
+                 "KVCache: k and v must be 4-dimensional and alike in shape, strides, dtype and device")
+        _require(k.dtype in _KV_FORMATS, f"KVCache: dtype {k.dtype} (bfloat16, float8_e4m3fn or int8)")
+        _require(k.is_cuda, "KVCache: GPU tensors only (there is no CPU path)")
+        n, h, cap, d = k.shape
+        _require(d in (64, 128), f"KVCache: head_dim {d} (64 or 128)")
+        _require(n > 0 and h > 0 and cap > 0, f"KVCache: empty shape {tuple(k.shape)}")
+        es = k.element_size()
+        _require(k.stride(3) == 1 and all(k.stride(i) * es % 16 == 0 for i in range(3) if k.shape[i] > 1) and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
+                 "KVCache: the last dimension must be contiguous and every row start at a multiple of 16 bytes")
+        stride = [k.stride(i) if k.shape[i] > 1 else 0 for i in range(3)]
+        sstride = [0, 0, 0]
+        if k.dtype == BF16:
+            _require(k_scale is None and v_scale is None, "KVCache: a bf16 cache has no scales")
+        else:
+            _require(k_scale is not None and v_scale is not None and k_scale.dtype == v_scale.dtype == torch.float32
+                     and tuple(k_scale.shape) == tuple(v_scale.shape) == (n, h, cap) and k_scale.stride() == v_scale.stride()
+                     and k_scale.device == v_scale.device == k.device,
+                     "KVCache: an 8-bit cache needs fp32 scales [n_seq, kv_heads, capacity] for k and v, alike in strides")
+            sstride = list(k_scale.stride())
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_seq, self.kv_heads, self.capacity, self.head_dim, self.dtype, self.device = n, h, cap, d, k.dtype, k.device
+        self._c = _lib.KvCache(format=_KV_FORMATS[k.dtype], n_seq=n, capacity=cap, kv_heads=h, head_dim=d, k=k.data_ptr(), v=v.data_ptr(),
+                               k_scale=k_scale.data_ptr() if k_scale is not None else None, v_scale=v_scale.data_ptr() if v_scale is not None else None,
+                               stride_seq=stride[0], stride_head=stride[1], stride_pos=stride[2],
+                               scale_stride_seq=sstride[0], scale_stride_head=sstride[1], scale_stride_pos=sstride[2])
+        self._ref = C.byref(self._c)
+
+    @classmethod
+    def empty(cls, n_seq: int, capacity: int, kv_heads: int, head_dim: int, dtype="e4m3", device="cuda") -> "KVCache":
+        """A zeroed cache; ``dtype`` "bf16", "e4m3", "int8" or the torch dtype."""
+        dt = KV_DTYPES.get(dtype, dtype)
+        _require(dt in _KV_FORMATS, f"KVCache: dtype {dtype!r} (one of {sorted(KV_DTYPES)})")
+        k, v = (torch.zeros(n_seq, kv_heads, capacity, head_dim, device=device, dtype=torch.uint8 if dt != BF16 else dt) for _ in range(2))
+        if dt == BF16:
+            return cls(k, v)
+        ks, vs = (torch.zeros(n_seq, kv_heads, capacity, device=device, dtype=torch.float32) for _ in range(2))
+        return cls(k.view(dt), v.view(dt), ks, vs)
+
+
+def _kv_source(cache: KVCache, k, v, what: str) -> int:
+    _require(k.dtype == v.dtype == BF16 and k.dim() == v.dim() == 2 and k.shape == v.shape and k.shape[1] == cache.kv_heads * cache.head_dim
+             and k.stride() == v.stride() and (k.stride(1) == 1 or k.shape[0] == 0),
+             f"{what}: k and v must be bf16 [tokens, kv_heads * head_dim] row-major views with the same strides")
+    _on_current_device(cache.k, k, v)
+    return k.stride(0)
+
+
+def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor) -> KVCache:
+    """Slot (sequence s, position t) of the cache takes row rows[s * capacity + t] (int32) of k / v (bf16 [tokens, kv_heads * head_dim]
+    views, e.g. columns of packed q|k|v rows), rounded to the cache's format; a row number below 0 or past the last token leaves the slot
+    as it is.  Several slots may name one row."""
+    ld = _kv_source(cache, k, v, "kv_write")
+    _i32(rows, cache.n_seq * cache.capacity, "kv_write: rows")
+    _on_current_device(rows)
+    check(_lib.load().spacer_kv_write(cache._ref, _ptr(k), _ptr(v), ld, k.shape[0], _ptr(rows), _stream()), "kv_write")
+    return cache
+
+
+def _kv_lengths(t: torch.Tensor, n: int, what: str) -> int:
+    """1 when ``t`` holds one length per sequence, 0 when one for all of them."""
+    _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() in (1, n), f"{what}: expected 1 or {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
+    _on_current_device(t)
+    return int(t.numel() == n and n > 1)
+
+
+def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor) -> KVCache:
+    """The newest N = tokens / n_seq tokens of every sequence: row s * N + i of k / v (as in ``kv_write``) goes to position lengths[s] + i
+    of sequence s (``lengths`` int32 on the device: [n_seq], or [1] for all).  Positions outside the cache are dropped."""
+    ld = _kv_source(cache, k, v, "kv_append")
+    _require(k.shape[0] % cache.n_seq == 0, f"kv_append: {k.shape[0]} rows for {cache.n_seq} sequences")
+    per = _kv_lengths(lengths, cache.n_seq, "kv_append: lengths")
+    check(_lib.load().spacer_kv_append(cache._ref, _ptr(k), _ptr(v), ld, k.shape[0] // cache.n_seq, _ptr(lengths), per, _stream()), "kv_append")
+    return cache
+
+
+def kv_read(cache: KVCache, lengths: Optional[torch.Tensor] = None, *, dtype=BF16):
+    """(k, v) [n_seq, capacity, kv_heads, head_dim] in bf16 or fp32: the values that the cache stands for.  ``lengths`` (int32 [n_seq]): positions at
+    and behind a sequence's length come back as zeros."""
+    _require(dtype in (BF16, torch.float32), f"kv_read: dtype {dtype} (bfloat16 or float32)")
+    _on_current_device(cache.k)
+    if lengths is not None:
+        _i32(lengths, cache.n_seq, "kv_read: lengths")
+        _on_current_device(lengths)
+    shape = (cache.n_seq, cache.capacity, cache.kv_heads, cache.head_dim)
+    k, v = torch.empty(shape, device=cache.device, dtype=dtype), torch.empty(shape, device=cache.device, dtype=dtype)
+    check(_lib.load().spacer_kv_read(cache._ref, _ptr(lengths), _ptr(k), _ptr(v), int(dtype == torch.float32), _stream()), "kv_read")
+    return k, v
+
+
+def decode_qkv_finish_cache(acc32, bias, cos, sin, q_out, cache: KVCache, tail_len, Hq, *, rowss=None, rowss_zero=None, norm_cols=0, eps=0.0):
+    """decode_qkv_finish (or with ``rowss``: decode_qkv_finish_normed) with K and V going to position ``tail_len`` of ``cache`` in its format."""
+    B, D = cache.n_seq, cache.head_dim
+    _require(acc32.dtype == torch.float32 and acc32.is_contiguous() and tuple(acc32.shape) == (B, (Hq + 2 * cache.kv_heads) * D)
+             and cos.shape == sin.shape == (B, D) and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+             and q_out.dtype == BF16 and q_out.is_contiguous() and tuple(q_out.shape) == (B, Hq * D),
+             "decode_qkv_finish_cache: acc32 fp32 [B, (Hq + 2 kv_heads) * D], cos / sin fp32 [B, D], q_out bf16 [B, Hq * D], all contiguous")
+    _on_current_device(acc32, bias, cos, sin, q_out, cache.k, rowss, rowss_zero)
+    per = _kv_lengths(tail_len, B, "decode_qkv_finish_cache: tail_len")
+    check(_lib.load().spacer_decode_qkv_finish_cache(_ptr(acc32), _ptr(bias), _ptr(cos), _ptr(sin), _ptr(q_out), cache._ref, _ptr(tail_len), per,
+                                                     _ptr(rowss), _ptr(rowss_zero), norm_cols, eps, Hq, _stream()), "decode_qkv_finish_cache")
+
+
+def attn_cache_workspace_bytes(prompt: Optional[KVCache], tail: Optional[KVCache], rows: int, B: int, nodes: int, Hq: int) -> int:
+    n = int(_lib.load().spacer_attn_cache_workspace_bytes(prompt._ref if prompt is not None else None, tail._ref if tail is not None else None, rows, B, nodes, Hq))
+    check(min(n, 0), "attn_cache_workspace_bytes")
+    return n
+
+
+def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache], tail_len, Hq, scale, *, rows_per_prompt=1, row0=None, nodes=1,
+               tree=None, out=None, workspace=None):
+    """Decode attention over caches in any format, for one new token per sequence (``nodes`` = 1) or a tree of up to 64 drafted tokens.
+
+    q bf16 [B * nodes, Hq * head_dim] (row b * nodes + i = node i of sequence b).  Node i sees its prompt's positions [0, prompt_len[p]), its
+    sequence's positions [0, tail_len[b]) in ``tail``, and the nodes j whose bit j is set in its mask, node j being at position tail_len[b] + j of
+    ``tail`` (append the nodes first: ``kv_append`` / ``decode_qkv_finish_cache``).  ``tree``: int64 [nodes] (one tree for all sequences) or
+    [B, nodes]; None: node i sees the nodes up to and including itself.  A node that sees nothing gets zeros.
+    ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` sequences from
+    p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt each.
+    prompt_len int32 [n_prompts]; tail_len int32 [B] or [1].  ``workspace``: attn_cache_workspace_bytes bytes; None allocates it."""
+    _require(prompt is not None or tail is not None, "attn_cache: a prompt or a tail cache is needed")
+    c = prompt if prompt is not None else tail
+    _require(q.dtype == BF16 and q.dim() == 2 and q.shape[1] == Hq * c.head_dim and q.stride(1) == 1 and nodes >= 1 and q.shape[0] % nodes == 0,
+             f"attn_cache: q must be bf16 [B * nodes, Hq * head_dim] with contiguous rows, got {tuple(q.shape)} {q.dtype}, {nodes} nodes")
+    B = q.shape[0] // nodes
+    _on_current_device(q, c.k, tail.k if tail is not None else None, row0, tree, out, workspace)
+    per = 0
+    if prompt is not None:
+        _i32(prompt_len, prompt.n_seq, "attn_cache: prompt_len")
+        _on_current_device(prompt_len)
+        if row0 is not None:
+            _i32(row0, prompt.n_seq + 1, "attn_cache: row0")
+    if tail is not None:
+        per = _kv_lengths(tail_len, B, "attn_cache: tail_len")
+    tree_per = 0
+    if tree is not None:
+        _require(tree.dtype == torch.int64 and tree.is_contiguous() and tuple(tree.shape) in ((nodes,), (B, nodes)),
+                 f"attn_cache: tree must be contiguous int64 [{nodes}] or [{B}, {nodes}], got {tuple(tree.shape)} {tree.dtype}")
+        tree_per = int(tree.dim() == 2)
+    if out is None:
+        out = torch.empty(q.shape[0], Hq * c.head_dim, device=q.device, dtype=BF16)
+    _require(out.dtype == BF16 and out.is_contiguous() and tuple(out.shape) == (q.shape[0], Hq * c.head_dim), "attn_cache: out must be contiguous bf16 [B * nodes, Hq * head_dim]")
+    if workspace is None:
+        workspace = torch.empty(attn_cache_workspace_bytes(prompt, tail, rows_per_prompt, B, nodes, Hq), device=q.device, dtype=torch.uint8)
+    check(_lib.load().spacer_attn_cache(_ptr(q), q.stride(0), prompt._ref if prompt is not None else None, _ptr(prompt_len) if prompt is not None else None,
+                                        _ptr(row0) if prompt is not None else None, rows_per_prompt, tail._ref if tail is not None else None,
+                                        _ptr(tail_len) if tail is not None else None, per, _ptr(tree), tree_per, _ptr(out), B, nodes, Hq, scale,
+                                        _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()), "attn_cache")
+    return out
+
+
+# ----------------------------------------------------------------------------------------- logits before the sampler
+def token_history(B: int, vocab: int, device):
+    """(seen, counts) of ``B`` rows without a token yet: the bit map int32 [B, ceil(vocab / 32)] and the counts int32 [B, vocab]."""
+    return (torch.zeros(B, (vocab + 31) // 32, device=device, dtype=torch.int32), torch.zeros(B, vocab, device=device, dtype=torch.int32))
+
+
+def _history(seen, counts, B, vocab, what):
+    _require(seen.dtype == torch.int32 and seen.is_contiguous() and tuple(seen.shape) == (B, (vocab + 31) // 32),
+             f"{what}: seen must be contiguous int32 [{B}, {(vocab + 31) // 32}], got {tuple(seen.shape)} {seen.dtype}")
+    _require(counts is None or (counts.dtype == torch.int32 and counts.is_contiguous() and tuple(counts.shape) == (B, vocab)),
+             f"{what}: counts must be contiguous int32 [{B}, {vocab}]")
+
+
+def token_history_add_(seen, counts, ids, lengths=None, *, vocab: Optional[int] = None):
+    """Marks ids[b, i] (int64 [B, n], i < lengths[b] where given) as seen in row b and counts them; ``counts`` None only marks (prompt tokens:
+    the repetition penalty asks what has been seen, the frequency and presence penalties what has been generated).  Ids outside the vocabulary
+    are skipped.  ``vocab``: needed without ``counts`` when it is not a multiple of 32."""
+    _require(ids.dtype == torch.int64 and ids.dim() == 2 and (ids.stride(1) == 1 or ids.shape[1] <= 1), f"token_history_add_: ids must be int64 [B, n] with contiguous rows, got {tuple(ids.shape)} {ids.dtype}")
+    B, n = ids.shape
+    vocab = vocab if vocab is not None else counts.shape[1] if counts is not None else seen.shape[1] * 32
+    _history(seen, counts, B, vocab, "token_history_add_")
+    if lengths is not None:
+        _i32(lengths, B, "token_history_add_: lengths")
+    _on_current_device(seen, counts, ids, lengths)
+    check(_lib.load().spacer_token_history_add(_ptr(seen), _ptr(counts), B, vocab, _ptr(ids), ids.stride(0), n, _ptr(lengths), _stream()), "token_history_add")
+
+
+def _per_row(x, neutral, B, what):
+    """(number, device pointer) of a penalty given as a number, an fp32 [B] tensor or None."""
+    if x is None:
+        return neutral, _ptr(None)
+    if isinstance(x, torch.Tensor):
+        _require(x.dtype == torch.float32 and x.is_contiguous() and tuple(x.shape) == (B,), f"process_logits: {what} must be a number or contiguous fp32 [{B}]")
+        _on_current_device(x)
+        return neutral, _ptr(x)
+    return float(x), _ptr(None)
+
+
+def process_logits(logits32, *, seen=None, counts=None, repetition=None, frequency=None, presence=None, bias=None, allowed=None, allowed_row=None,
+                   out=None):
+    """Logits of a decode step made ready for the sampler, into ``out`` (None: in place):
+        x = x / repetition if x > 0 else x * repetition    on tokens marked in ``seen``
+        x = x - frequency * count - presence * (count > 0)  with ``counts``
+        x = x + bias                                        fp32 [vocab] or [B, vocab]
+        x = -inf                                            where the token's bit in the row's ``allowed`` mask is clear
+    repetition / frequency / presence: numbers or fp32 [B].  allowed: int32 [n_masks, ceil(vocab / 32)] (bit v % 32 of word v // 32); row b
+    takes mask allowed_row[b] (int32 [B], a number outside the table: no mask), or without ``allowed_row`` mask b, or the only one.  A row whose
+    mask allows nothing is all -inf: the sampler has nothing to draw there."""
+    _require(logits32.dtype == torch.float32 and logits32.dim() == 2 and logits32.stride(1) == 1, "process_logits: logits must be fp32 [B, vocab] with contiguous rows")
+    B, vocab = logits32.shape
+    if out is None:
+        out = logits32
+    _require(out.dtype == torch.float32 and out.shape == logits32.shape and out.stride(1) == 1, "process_logits: out must be fp32 [B, vocab] with contiguous rows")
+    if seen is not None:
+        _history(seen, counts, B, vocab, "process_logits")
+    _require(seen is not None or (counts is None and repetition is None), "process_logits: penalties need the history (seen)")
+    words, ld_bias, n_masks = (vocab + 31) // 32, 0, 0
+    if bias is not None:
+        _require(bias.dtype == torch.float32 and tuple(bias.shape) in ((vocab,), (B, vocab)) and bias.stride(-1) == 1,
+                 f"process_logits: bias must be fp32 [{vocab}] or [{B}, {vocab}] with contiguous rows, got {tuple(bias.shape)} {bias.dtype}")
+        ld_bias = bias.stride(0) if bias.dim() == 2 else 0
+    if allowed is not None:
+        _require(allowed.dtype == torch.int32 and allowed.dim() == 2 and allowed.is_contiguous() and allowed.shape[1] == words,
+                 f"process_logits: allowed must be contiguous int32 [n_masks, {words}], got {tuple(allowed.shape)} {allowed.dtype}")
+        n_masks = allowed.shape[0]
+        if allowed_row is not None:
+            _i32(allowed_row, B, "process_logits: allowed_row")
+    else:
+        _require(allowed_row is None, "process_logits: allowed_row without allowed")
+    _on_current_device(logits32, out, seen, counts, bias, allowed, allowed_row)
+    r, rp = _per_row(repetition, 1.0, B, "repetition")
+    f, fp = _per_row(frequency, 0.0, B, "frequency")
+    p, pp = _per_row(presence, 0.0, B, "presence")
+    check(_lib.load().spacer_process_logits(_ptr(logits32), logits32.stride(0), _ptr(out), out.stride(0), B, vocab, _ptr(seen), _ptr(counts), r, rp, f, fp, p, pp,
+                                            _ptr(bias), ld_bias, _ptr(allowed), n_masks, _ptr(allowed_row), _stream()), "process_logits")
+    return out
+
+
 # ----------------------------------------------------------------------------------------- element-wise
 def swiglu_fwd(gu, *, out=None):
     rows, two_i = gu.shape

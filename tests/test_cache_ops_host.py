@@ -1,0 +1,119 @@
+"""Refusals of the cache and logits operators, and the layout of spacer_kv_cache: host only, no kernel is launched."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+from spacer_amd import _lib
+from spacer_amd import kernels as K
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+EINVAL, ENOMEM = -1, -3
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    return _lib.load()
+
+
+def test_struct_layout(tmp_path):
+    names = [f for f, _ in _lib.KvCache._fields_]
+    src = '#include <stdio.h>\n#include <stddef.h>\n#include "%s"\nint main(void) { printf("%%zu", sizeof(spacer_kv_cache));\n' % os.path.join(ROOT, "include", "spacer_hip.h")
+    src += "".join(f'printf(" %zu", offsetof(spacer_kv_cache, {n}));\n' for n in names) + "return 0; }\n"
+    (tmp_path / "p.c").write_text(src)
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-o", str(tmp_path / "p"), str(tmp_path / "p.c")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "p")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [C.sizeof(_lib.KvCache)] + [getattr(_lib.KvCache, n).offset for n in names]
+
+
+def cache(**kw):
+    """A well-formed description of memory that is never touched."""
+    f = dict(format=_lib.SPACER_KV_INT8, n_seq=2, capacity=64, kv_heads=2, head_dim=128, k=0x1000, v=0x2000, k_scale=0x3000, v_scale=0x4000,
+             stride_seq=2 * 64 * 128, stride_head=64 * 128, stride_pos=128, scale_stride_seq=128, scale_stride_head=64, scale_stride_pos=1)
+    f.update(kw)
+    c = _lib.KvCache(**{k: v for k, v in f.items() if k != "struct_bytes"})
+    if "struct_bytes" in kw:
+        c.struct_bytes = kw["struct_bytes"]
+    return c
+
+
+BAD_CACHES = [dict(struct_bytes=8), dict(format=3), dict(format=-1), dict(head_dim=80), dict(head_dim=0), dict(n_seq=0), dict(capacity=-1), dict(kv_heads=0),
+              dict(k=None), dict(v=0x2008), dict(stride_pos=136), dict(stride_head=8), dict(k_scale=None), dict(v_scale=None),
+              dict(format=_lib.SPACER_KV_BF16, stride_pos=132)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES)
+def test_bad_caches_are_refused(lib, bad):
+    c, good, p = cache(**bad), cache(), 0x10000
+    assert lib.spacer_kv_write(C.byref(c), p, p, 256, 4, p, None) == EINVAL
+    assert lib.spacer_kv_append(C.byref(c), p, p, 256, 1, p, 0, None) == EINVAL
+    assert lib.spacer_kv_read(C.byref(c), None, p, p, 0, None) == EINVAL
+    assert lib.spacer_decode_qkv_finish_cache(p, None, p, p, p, C.byref(c), p, 0, None, None, 0, 0.0, 4, None) == EINVAL
+    assert lib.spacer_attn_cache(p, 512, C.byref(c), p, None, 1, None, None, 0, None, 0, p, 2, 1, 4, 1.0, p, 1 << 30, None) == EINVAL
+    assert lib.spacer_attn_cache(p, 512, None, None, None, 1, C.byref(c), p, 0, None, 0, p, 2, 1, 4, 1.0, p, 1 << 30, None) == EINVAL
+    assert lib.spacer_attn_cache_workspace_bytes(C.byref(good), C.byref(c), 1, 2, 1, 4) == -1
+    assert lib.spacer_last_error()
+
+
+def test_entries_refuse(lib):
+    c, p = cache(), 0x10000
+    r = C.byref(c)
+    assert lib.spacer_kv_write(None, p, p, 256, 4, p, None) == EINVAL
+    assert lib.spacer_kv_write(r, p, p, 256, 4, None, None) == EINVAL
+    assert lib.spacer_kv_write(r, p, p, 256, -1, p, None) == EINVAL
+    assert lib.spacer_kv_write(r, p + 2, p, 256, 4, p, None) == EINVAL
+    assert lib.spacer_kv_write(r, p, p, 260, 4, p, None) == EINVAL
+    assert lib.spacer_kv_append(r, p, p, 256, 1, None, 0, None) == EINVAL
+    assert lib.spacer_kv_append(r, p, p, 256, 1 << 30, p, 0, None) == EINVAL
+    assert lib.spacer_kv_read(r, None, p, None, 0, None) == EINVAL
+    assert lib.spacer_kv_read(r, None, p + 4, p, 0, None) == EINVAL
+
+    def attn(q=p, ld=512, prompt=r, plen=p, row0=None, rows=1, tail=r, tlen=p, o=p, B=2, N=1, Hq=4, ws=p, n=1 << 30):
+        return lib.spacer_attn_cache(q, ld, prompt, plen, row0, rows, tail, tlen, 0, None, 0, o, B, N, Hq, 1.0, ws, n, None)
+    for kw in (dict(q=None), dict(q=p + 8), dict(ld=516), dict(prompt=None, tail=None), dict(plen=None), dict(tlen=None), dict(o=None), dict(B=3), dict(B=-1), dict(N=0), dict(N=65),
+               dict(Hq=3), dict(Hq=0), dict(rows=0), dict(rows=2), dict(prompt=C.byref(cache(head_dim=64))), dict(prompt=C.byref(cache(format=1))),
+               dict(prompt=C.byref(cache(kv_heads=1)))):
+        assert attn(**kw) == EINVAL, kw
+    assert attn(ws=None) == ENOMEM and attn(n=64) == ENOMEM and attn(ws=p + 4) == ENOMEM
+    need = lib.spacer_attn_cache_workspace_bytes(r, r, 1, 2, 1, 4)
+    assert need > 0 and attn(n=need - 1) == ENOMEM
+
+    def logits(x=p, out=p, B=2, V=100, seen=p, counts=p, rep=1.0, f=0.0, pr=0.0, allowed=None, n=0, row=None):
+        return lib.spacer_process_logits(x, 100, out, 100, B, V, seen, counts, rep, None, f, None, pr, None, None, 0, allowed, n, row, None)
+    for kw in (dict(x=None), dict(out=None), dict(V=0), dict(B=-1), dict(B=70000), dict(rep=0.0), dict(rep=-1.0), dict(rep=float("nan")), dict(seen=None), dict(counts=None, f=0.1),
+               dict(counts=None, pr=0.1), dict(allowed=p, n=3), dict(allowed=p, n=0, row=p)):
+        assert logits(**kw) == EINVAL, kw
+    assert logits(B=0) == 0
+    assert lib.spacer_token_history_add(None, None, 2, 100, p, 4, 4, None, None) == EINVAL
+    assert lib.spacer_token_history_add(p, None, 2, 0, p, 4, 4, None, None) == EINVAL
+    assert lib.spacer_token_history_add(p, None, 2, 100, None, 4, 4, None, None) == EINVAL
+    assert lib.spacer_token_history_add(p, None, 2, 100, p, 4, 0, None, None) == 0
+
+
+def test_python_layer_refuses():
+    z = torch.zeros(1, 2, 16, 128, dtype=torch.int8)
+    s = torch.zeros(1, 2, 16)
+    with pytest.raises(K.SpacerError, match="GPU"):
+        K.KVCache(z, z, s, s)
+    with pytest.raises(K.SpacerError, match="alike"):
+        K.KVCache(z, z[:, :1], s, s)
+    with pytest.raises(K.SpacerError, match="dtype"):
+        K.KVCache(z.half(), z.half(), s, s)
+    with pytest.raises(K.SpacerError, match="dtype"):
+        K.KVCache.empty(1, 2, 3, 128, "fp4", device="cpu")
+    with pytest.raises(K.SpacerError, match="fp32"):
+        K.process_logits(torch.zeros(2, 10, dtype=torch.float16))
+    with pytest.raises(K.SpacerError, match="history"):
+        K.process_logits(torch.zeros(2, 10), repetition=1.1)
+    with pytest.raises(K.SpacerError, match="allowed_row"):
+        K.process_logits(torch.zeros(2, 10), allowed_row=torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(K.SpacerError, match="bias"):
+        K.process_logits(torch.zeros(2, 10), bias=torch.zeros(9))
+    with pytest.raises(K.SpacerError, match="ids"):
+        K.token_history_add_(torch.zeros(2, 1, dtype=torch.int32), None, torch.zeros(2, 4, dtype=torch.int32))
+    with pytest.raises(K.SpacerError, match="cache"):
+        K.attn_cache(torch.zeros(2, 128, dtype=torch.bfloat16), None, None, None, None, 1, 1.0)
