@@ -84,87 +84,109 @@ constexpr int lds_bytes(int es, int D, int nc) {
     return work > join ? work : join;
 }
 
-// One workgroup's range of keys [t0, t1) (in 32-key tiles) of `total` keys x 16 NC columns from c0 on, and its record.
-//   col_info(c, row, head, node): the query of column c, or false
-//   base: first key that the mask bits speak of (= total where there are none)
-template <int FMT, int D, int NC, class ColInfo>
-__device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const char* vp, const float* ksp, const float* vsp, long s_pos, long c_pos,
-                       int total, int base, int t0, int t1, int c0, int slot, ColInfo col_info) {
-    using T = Tile<FMT, D, NC>;
-    constexpr int DF = D / 16;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, g = lane >> 4;
-    const long row_b = s_pos * T::ES;
-    const long ncol_all = (long)A.B * A.N * A.Hq;
-    char* vimg = smem + wave * T::IMG;
-    float* sc = (float*)(smem + 4 * T::IMG) + wave * 2 * TK;
-    char* qlds = smem + 4 * (T::IMG + 2 * TK * 4);
+// Keys [0, total) of one (sequence, kv head), this workgroup's share of them, and the first key that the nodes' masks speak of (total: none)
+struct KeySegment {
+    const char *k, *v;
+    const float *ks, *vs;
+    int row_b, c_pos;                 // bytes between positions, floats between their scales
+    int total, base, t0, t1;          // t0, t1: in 32-key tiles
+};
 
-    // ---- queries: fragment (cb, step) = for column l15 the 8 numbers that step's slots of lane group g stand for
-    auto q_frag = [&](int cb, int step) -> bf16x8 {
+// The state of one workgroup's 16 NC columns and what it does with a segment of keys.  ColInfo: (c, row, head, node) -> the query of column c, or false.
+template <int FMT, int D, int NC, class ColInfo>
+struct Columns {
+    using T = Tile<FMT, D, NC>;
+    static constexpr int DF = D / 16, QR = NC <= 2 ? NC : 1;
+
+    const AttnCacheArgs& A;
+    const ColInfo& info;
+    const int c0, lane, wave, l15, g;
+    char *vimg, *qlds;
+    float* sc;
+    bf16x8 qreg[QR][T::STEPS];
+    f32x4 oacc[NC][DF];
+    float m_run[NC], l_run[NC];
+    uint4 kr[2][T::KL], vr[T::VL];
+    float scr;
+
+    __device__ __forceinline__ Columns(const AttnCacheArgs& args, const ColInfo& ci, char* smem, int first)
+        : A(args), info(ci), c0(first), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
+          g((threadIdx.x & 63) >> 4), scr(0.f) {
+        vimg = smem + wave * T::IMG;
+        sc = (float*)(smem + 4 * T::IMG) + wave * 2 * TK;
+        qlds = smem + 4 * (T::IMG + 2 * TK * 4);
+#pragma unroll
+        for (int cb = 0; cb < NC; ++cb) {
+            m_run[cb] = -INFINITY; l_run[cb] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DF; ++d) oacc[cb][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // fragment (cb, step): for column l15 the 8 numbers that the step's slots of lane group g stand for
+    __device__ __forceinline__ bf16x8 q_frag(int cb, int step) const {
         int row, head, node;
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (col_info(c0 + cb * 16 + l15, row, head, node)) {
+        if (info(c0 + cb * 16 + l15, row, head, node)) {
             const int d = T::ES == 2 ? step * 32 + g * 8 : (step >> 1) * 64 + g * 16 + (step & 1) * 8;
             x = *(const uint4*)(A.q + ((long)row * A.N + node) * A.q_ld + (long)head * D + d);
         }
         return __builtin_bit_cast(bf16x8, x);
-    };
-    bf16x8 qreg[NC <= 2 ? NC : 1][T::STEPS];
-    if (NC <= 2) {
-#pragma unroll
-        for (int cb = 0; cb < (NC <= 2 ? NC : 1); ++cb)
-#pragma unroll
-            for (int s = 0; s < T::STEPS; ++s) qreg[cb][s] = q_frag(cb, s);
-    } else {
-        for (int f = wave; f < NC * T::STEPS; f += 4) *(bf16x8*)(qlds + (f * 64 + lane) * 16) = q_frag(f / T::STEPS, f % T::STEPS);
-        __syncthreads();
     }
-    uint64_t see[NC];                                     // nodes that the column's node sees
+    __device__ __forceinline__ void load_queries() {
+        if (NC <= 2) {
 #pragma unroll
-    for (int cb = 0; cb < NC; ++cb) {
-        int row, head, node;
-        see[cb] = 0;
-        if (base < total && col_info(c0 + cb * 16 + l15, row, head, node))
-            see[cb] = A.tree ? (uint64_t)A.tree[(long)row * A.tree_stride + node] : (node >= 63 ? ~0ull : (2ull << node) - 1);
+            for (int cb = 0; cb < QR; ++cb)
+#pragma unroll
+                for (int s = 0; s < T::STEPS; ++s) qreg[cb][s] = q_frag(cb, s);
+        } else {
+            for (int f = wave; f < NC * T::STEPS; f += 4) *(bf16x8*)(qlds + (f * 64 + lane) * 16) = q_frag(f / T::STEPS, f % T::STEPS);
+            __syncthreads();
+        }
     }
-    f32x4 oacc[NC][DF];
-    float m_run[NC], l_run[NC];
-#pragma unroll
-    for (int cb = 0; cb < NC; ++cb) {
-        m_run[cb] = -INFINITY; l_run[cb] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DF; ++d) oacc[cb][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-    const float kmul = A.scale * LOG2E;
 
-    uint4 kr[2][T::KL], vr[T::VL];
-    float scr = 0.f;
-    auto fetch = [&](int t) {                             // (keys behind the last repeat it: always inside the cache)
-        const int k0 = t * TK, last = total - 1;
+    // requests tile t: 64-bit arithmetic stays in scalars, a lane adds 32 bits (32 rows span less than 2^31 bytes: checked on the host).
+    // Keys behind the last repeat it, so every address lies inside the cache.
+    __device__ __forceinline__ void fetch(const KeySegment& s, int t) {
+        const int k0 = t * TK, last = s.total - 1 - k0;
+        const char *kb = s.k + (long)k0 * s.row_b, *vb = s.v + (long)k0 * s.row_b;
+        const bool full = last >= TK - 1;
 #pragma unroll
         for (int kf = 0; kf < 2; ++kf) {
-            const char* p = kp + min(k0 + kf * 16 + l15, last) * row_b + g * 16;
+            const uint32_t off = (uint32_t)((full ? kf * 16 + l15 : min(kf * 16 + l15, last)) * s.row_b + g * 16);
 #pragma unroll
-            for (int h = 0; h < T::KL; ++h) kr[kf][h] = *(const uint4*)(p + h * 64);
+            for (int h = 0; h < T::KL; ++h) kr[kf][h] = *(const uint4*)(kb + off + h * 64);
         }
-        if (FMT != KV_BF16) scr = (lane < TK ? ksp : vsp)[min(k0 + (lane & 31), last) * c_pos];
+        if (FMT != KV_BF16) {
+            const float* sb = (lane < TK ? s.ks : s.vs) + (long)k0 * s.c_pos;
+            scr = sb[min(lane & (TK - 1), last) * s.c_pos];
+        }
 #pragma unroll
-        for (int i = 0; i < T::VL; ++i)
-            vr[i] = *(const uint4*)(vp + min(k0 + lane / T::CPR + i * (64 / T::CPR), last) * row_b + (lane % T::CPR) * 16);
-    };
+        for (int i = 0; i < T::VL; ++i) {
+            const int row = lane / T::CPR + i * (64 / T::CPR);
+            vr[i] = *(const uint4*)(vb + (uint32_t)((full ? row : min(row, last)) * s.row_b + (lane % T::CPR) * 16));
+        }
+    }
 
-    if (t0 + wave < t1) fetch(t0 + wave);
-    for (int t = t0 + wave; t < t1; t += 4) {
+    // tiles first, first + 4, ... < s.t1 of a segment; the tile `first` has been requested by fetch()
+    __device__ __forceinline__ void run(const KeySegment& s, int first) {
+        int t = first;
+        const int plain = min(s.t1, s.base / TK);         // from here on some key of a tile is a node or lies behind the last key
+        for (; t < plain; t += 4) tile<false>(s, t);
+        for (; t < s.t1; t += 4) tile<true>(s, t);
+    }
+
+    template <bool EDGE>
+    __device__ __forceinline__ void tile(const KeySegment& s, int t) {
         const int k0 = t * TK;
-        const bool edge = k0 + TK > base;                 // some key of the tile is a node or lies behind the last key
-        asm volatile("" ::: "memory");                    // (the previous step's LDS reads stay in front of these writes: LDS is in order)
-        if (FMT != KV_BF16) sc[lane] = lane < TK ? scr * kmul : scr;
+        asm volatile("" ::: "memory");                    // (the previous tile's LDS reads stay in front of these writes: LDS is in order)
+        if (FMT != KV_BF16) sc[lane] = lane < TK ? scr * (A.scale * LOG2E) : scr;
         bool odd_v = false;                               // a NaN or an infinity in a bf16 V row that some columns must not see
 #pragma unroll
         for (int i = 0; i < T::VL; ++i) {
             const int row = lane / T::CPR + i * (64 / T::CPR);
             *(uint4*)(vimg + row * T::RB + (((lane % T::CPR) ^ T::swz(row)) * 16)) = vr[i];
-            if (FMT == KV_BF16 && edge) {
+            if (FMT == KV_BF16 && EDGE) {
                 const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) odd_v |= amax2(w[e]) >= 0x7f80u;
@@ -175,24 +197,24 @@ __device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const
 #pragma unroll
         for (int cb = 0; cb < NC; ++cb) st[cb][0] = st[cb][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < T::STEPS; ++s) {
+        for (int step = 0; step < T::STEPS; ++step) {
             bf16x8 kf8[2];
 #pragma unroll
             for (int kf = 0; kf < 2; ++kf) {
-                if (FMT == KV_BF16) kf8[kf] = __builtin_bit_cast(bf16x8, kr[kf][s]);
+                if (FMT == KV_BF16) kf8[kf] = __builtin_bit_cast(bf16x8, kr[kf][FMT == KV_BF16 ? step : 0]);
                 else {
-                    const uint4 x = kr[kf][s >> 1];
-                    kf8[kf] = codes_to_bf16<FMT>((s & 1) ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
+                    const uint4 x = kr[kf][FMT == KV_BF16 ? 0 : step >> 1];
+                    kf8[kf] = codes_to_bf16<FMT>((step & 1) ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
                 }
             }
 #pragma unroll
             for (int cb = 0; cb < NC; ++cb) {
-                const bf16x8 qf = NC <= 2 ? qreg[NC <= 2 ? cb : 0][s] : *(const bf16x8*)(qlds + ((cb * T::STEPS + s) * 64 + lane) * 16);
+                const bf16x8 qf = NC <= 2 ? qreg[NC <= 2 ? cb : 0][step] : *(const bf16x8*)(qlds + ((cb * T::STEPS + step) * 64 + lane) * 16);
                 st[cb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[0], qf, st[cb][0], 0, 0, 0);
                 st[cb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[1], qf, st[cb][1], 0, 0, 0);
             }
         }
-        if (t + 4 < t1) fetch(t + 4);                     // the registers of K and V are free: the next tile is under way during the rest
+        if (t + 4 < s.t1) fetch(s, t + 4);                // the registers of K and V are free: the next tile is under way during the rest
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // image and scales complete before any lane reads them
         __builtin_amdgcn_wave_barrier();
         float ksv[2][4], vsv[2][4];
@@ -207,16 +229,28 @@ __device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const
         // ---- online softmax in the log2 domain; the running maximum follows only in steps of more than 2^8 (weights stay below 2^8, far
         //      inside fp32 and bf16), so that O is rescaled a few times per range and not once per tile
         bf16x8 pf[NC];
-        auto visible = [&](int cb, int key) -> bool { return key < base || (key < total && ((see[cb] >> (key - base)) & 1)); };
+        uint64_t see[NC];
+        auto visible = [&](int cb, int key) -> bool { return key < s.base || (key < s.total && ((see[cb] >> (key - s.base)) & 1)); };
 #pragma unroll
         for (int cb = 0; cb < NC; ++cb) {
+            bool vis[2][4];
+            if (EDGE) {                                   // nodes that the column's node sees
+                int row, head, node;
+                see[cb] = 0;
+                if (s.base < s.total && info(c0 + cb * 16 + l15, row, head, node))
+                    see[cb] = A.tree ? (uint64_t)A.tree[(long)row * A.tree_stride + node] : (node >= 63 ? ~0ull : (2ull << node) - 1);
+#pragma unroll
+                for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) vis[kf][r] = visible(cb, k0 + kf * 16 + g * 4 + r);
+            }
             float p[2][4], mx = -INFINITY;
 #pragma unroll
             for (int kf = 0; kf < 2; ++kf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float x = st[cb][kf][r] * (FMT == KV_BF16 ? kmul : ksv[kf][r]);
-                    if (edge && !visible(cb, k0 + kf * 16 + g * 4 + r)) x = -INFINITY;
+                    float x = st[cb][kf][r] * (FMT == KV_BF16 ? A.scale * LOG2E : ksv[kf][r]);
+                    if (EDGE && !vis[kf][r]) x = -INFINITY;
                     p[kf][r] = x;
                     mx = fmaxf(mx, x);
                 }
@@ -229,7 +263,7 @@ __device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const
 #pragma unroll
                 for (int d = 0; d < DF; ++d) oacc[cb][d] *= alpha;
             }
-            const float m = m_run[cb] == -INFINITY ? 0.f : m_run[cb];     // nothing seen yet: every weight is 0
+            const float m = EDGE && m_run[cb] == -INFINITY ? 0.f : m_run[cb];     // nothing seen yet: every weight is 0
             float sum = 0.f;
 #pragma unroll
             for (int kf = 0; kf < 2; ++kf)
@@ -239,14 +273,15 @@ __device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const
                     sum += p[kf][r];
                     if (FMT != KV_BF16) {
                         p[kf][r] *= vsv[kf][r];
-                        if (edge && !visible(cb, k0 + kf * 16 + g * 4 + r)) p[kf][r] = 0.f;    // (the scale of a hidden row may be NaN)
+                        if (EDGE && !vis[kf][r]) p[kf][r] = 0.f;    // (the scale of a hidden row may be NaN)
                     }
                 }
             l_run[cb] += sum;
             pf[cb] = __builtin_bit_cast(bf16x8, make_uint4(pack_bf2(p[0][0], p[0][1]), pack_bf2(p[0][2], p[0][3]), pack_bf2(p[1][0], p[1][1]), pack_bf2(p[1][2], p[1][3])));
         }
         // ---- O^T += V^T . P^T; slot j of lane group g is key (j >> 2) * 16 + 4 g + (j & 3)
-        if (FMT == KV_BF16 && __any(odd_v)) {             // rare: a product with a hidden NaN or infinity would be NaN; add visible keys one by one
+        if (FMT == KV_BF16 && EDGE && __any(odd_v)) {     // rare: a product with a hidden NaN or infinity would be NaN; add visible keys one by one
+#pragma unroll 1
             for (int key = 0; key < TK; ++key)
 #pragma unroll
                 for (int cb = 0; cb < NC; ++cb) {
@@ -265,7 +300,7 @@ __device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const
                             if (on) oacc[cb][df][r] += w * x;
                         }
                 }
-            continue;
+            return;
         }
 #pragma unroll
         for (int df = 0; df < DF; ++df) {
@@ -290,44 +325,75 @@ __device__ void attend(const AttnCacheArgs& A, char* smem, const char* kp, const
         }
     }
 
-    // ---- join the waves, one block of 16 columns at a time: [wave][column][D + 4 floats], [wave][column] (m, l)
-    float* jo = (float*)smem;
-    float2* jm = (float2*)(smem + 4 * 16 * (D + 4) * 4);
-    constexpr int PER = D / 16;                           // floats per thread
-    const int jc = tid >> 4, jd = (tid & 15) * PER;
+    // joins the waves, one block of 16 columns at a time ([wave][column][D + 4 floats], [wave][column] (m, l) in LDS), and writes the record `slot` of
+    // every column, or with slot < 0 its output
+    __device__ __forceinline__ void finish(char* smem, int slot) {
+        const int tid = threadIdx.x;
+        float* jo = (float*)smem;
+        float2* jm = (float2*)(smem + 4 * 16 * (D + 4) * 4);
+        constexpr int PER = D / 16;                           // floats per thread
+        const int jc = tid >> 4, jd = (tid & 15) * PER;
+        const long ncol_all = (long)A.B * A.N * A.Hq;
 #pragma unroll
-    for (int cb = 0; cb < NC; ++cb) {
-        __syncthreads();
-        float l = l_run[cb];
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
+        for (int cb = 0; cb < NC; ++cb) {
+            __syncthreads();
+            float l = l_run[cb];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
 #pragma unroll
-        for (int df = 0; df < DF; ++df)
-            *(float4*)(jo + (wave * 16 + l15) * (D + 4) + df * 16 + g * 4) = make_float4(oacc[cb][df][0], oacc[cb][df][1], oacc[cb][df][2], oacc[cb][df][3]);
-        if (g == 0) jm[wave * 16 + l15] = make_float2(m_run[cb], l);
-        __syncthreads();
-        int row, head, node;
-        if (!col_info(c0 + cb * 16 + jc, row, head, node)) continue;
-        float M = -INFINITY;
+            for (int df = 0; df < DF; ++df)
+                *(float4*)(jo + (wave * 16 + l15) * (D + 4) + df * 16 + g * 4) = make_float4(oacc[cb][df][0], oacc[cb][df][1], oacc[cb][df][2], oacc[cb][df][3]);
+            if (g == 0) jm[wave * 16 + l15] = make_float2(m_run[cb], l);
+            __syncthreads();
+            int row, head, node;
+            if (!info(c0 + cb * 16 + jc, row, head, node)) continue;
+            float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * 16 + jc].x);
-        float L = 0.f, O[PER];
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * 16 + jc].x);
+            float L = 0.f, O[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) O[i] = 0.f;
+            for (int i = 0; i < PER; ++i) O[i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float2 ml = jm[w * 16 + jc];
-            const float f = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
-            L += ml.y * f;
+            for (int w = 0; w < 4; ++w) {
+                const float2 ml = jm[w * 16 + jc];
+                const float f = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+                L += ml.y * f;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) O[i] += jo[(w * 16 + jc) * (D + 4) + jd + i] * f;
+                for (int i = 0; i < PER; ++i) O[i] += jo[(w * 16 + jc) * (D + 4) + jd + i] * f;
+            }
+            const long col = ((long)row * A.N + node) * A.Hq + head;
+            if (slot < 0) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+                for (int i = 0; i < PER; i += 4)
+                    *(uint2*)(A.o + col * D + jd + i) = make_uint2(pack_bf2(O[i] * inv, O[i + 1] * inv), pack_bf2(O[i + 2] * inv, O[i + 3] * inv));
+                continue;
+            }
+            float* ro = A.rec_o + ((long)slot * ncol_all + col) * D + jd;
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) *(float4*)(ro + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
+            if ((tid & 15) == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
         }
-        const long col = ((long)row * A.N + node) * A.Hq + head;
-        float* ro = A.rec_o + ((long)slot * ncol_all + col) * D + jd;
-#pragma unroll
-        for (int i = 0; i < PER; i += 4) *(float4*)(ro + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
-        if ((tid & 15) == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
     }
+};
+
+template <int FMT>
+__device__ __forceinline__ KeySegment segment_of(const KvView& c, int seq, int hk, int total, int base, int splits, int sp) {
+    KeySegment s;
+    const long kv = ((long)seq * c.s_seq + (long)hk * c.s_head) * kv_size<FMT>(), ks = (long)seq * c.c_seq + (long)hk * c.c_head;
+    s.k = c.k + kv; s.v = c.v + kv; s.ks = c.ks + ks; s.vs = c.vs + ks;
+    s.row_b = (int)(c.s_pos * kv_size<FMT>()); s.c_pos = (int)c.c_pos;
+    s.total = total; s.base = base;
+    const int nt = (total + TK - 1) / TK, per = (nt + splits - 1) / splits;
+    s.t0 = sp * per; s.t1 = min(nt, s.t0 + per);
+    return s;
+}
+
+// rows [r0, r1) of the batch that prompt pr serves
+__device__ __forceinline__ void rows_of(const AttnCacheArgs& A, int pr, int& r0, int& r1) {
+    r0 = A.row0 ? min(max(A.row0[pr], 0), A.B) : min(pr * A.rows, A.B);
+    r1 = A.row0 ? min(max(A.row0[pr + 1], r0), A.B) : min((pr + 1) * A.rows, A.B);
+    r1 = min(r1, r0 + A.rows);
 }
 
 template <int FMT, int D, int NCA, int NCB>
@@ -341,33 +407,40 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
     if (role_a) {
         const int sp = job % A.sa, hk = (job / A.sa) % A.Hkv, pr = job / (A.sa * A.Hkv);
         if (pr >= A.n_prompts) return;
-        const int r0 = A.row0 ? min(max(A.row0[pr], 0), A.B) : min(pr * A.rows, A.B);
-        const int r1 = A.row0 ? min(max(A.row0[pr + 1], r0), A.B) : min((pr + 1) * A.rows, A.B);
-        const int nrow = min(r1 - r0, A.rows), ncol = nrow * A.N * rep, c0 = cb * 16 * NCA;
+        int r0, r1;
+        rows_of(A, pr, r0, r1);
+        const int per_row = A.N * rep, ncol = (r1 - r0) * per_row, c0 = cb * 16 * NCA;
         if (c0 >= ncol) return;
         const int total = min(max(A.prompt_len[pr], 0), A.prompt.cap);
-        const int nt = (total + TK - 1) / TK, per = (nt + A.sa - 1) / A.sa, t0 = sp * per, t1 = min(nt, t0 + per);
-        const long kv = ((long)pr * A.prompt.s_seq + (long)hk * A.prompt.s_head) * kv_size<FMT>(), ks = (long)pr * A.prompt.c_seq + (long)hk * A.prompt.c_head;
-        const int per_row = A.N * rep;
-        attend<FMT, D, NCA>(A, smem, A.prompt.k + kv, A.prompt.v + kv, A.prompt.ks + ks, A.prompt.vs + ks, A.prompt.s_pos, A.prompt.c_pos, total, total, t0,
-                            t1, c0, sp, [&](int c, int& row, int& head, int& node) -> bool {
-                                const int r = c / per_row, x = c - r * per_row;
-                                row = r0 + r; node = x / rep; head = hk * rep + x - node * rep;
-                                return c < ncol;
-                            });
+        const KeySegment s = segment_of<FMT>(A.prompt, pr, hk, total, total, A.sa, sp);
+        auto info = [&](int c, int& row, int& head, int& node) -> bool {
+            const int r = c / per_row, x = c - r * per_row;
+            row = r0 + r; node = x / rep; head = hk * rep + x - node * rep;
+            return c < ncol;
+        };
+        Columns<FMT, D, NCA, decltype(info)> W(A, info, smem, c0);
+        const int first = s.t0 + W.wave;
+        if (first < s.t1) W.fetch(s, first);
+        W.load_queries();
+        W.run(s, first);
+        W.finish(smem, sp);
     } else {
         const int sp = job % A.sb, hk = (job / A.sb) % A.Hkv, b = job / (A.sb * A.Hkv);
         if (b >= A.B) return;
         const int ncol = A.N * rep, c0 = cb * 16 * NCB;
         if (c0 >= ncol) return;
         const int base = min(max(A.tail_len[(long)b * A.len_stride], 0), A.tail.cap), total = min(base + A.N, A.tail.cap);
-        const int nt = (total + TK - 1) / TK, per = (nt + A.sb - 1) / A.sb, t0 = sp * per, t1 = min(nt, t0 + per);
-        const long kv = ((long)b * A.tail.s_seq + (long)hk * A.tail.s_head) * kv_size<FMT>(), ks = (long)b * A.tail.c_seq + (long)hk * A.tail.c_head;
-        attend<FMT, D, NCB>(A, smem, A.tail.k + kv, A.tail.v + kv, A.tail.ks + ks, A.tail.vs + ks, A.tail.s_pos, A.tail.c_pos, total, base, t0, t1, c0,
-                            A.sa + sp, [&](int c, int& row, int& head, int& node) -> bool {
-                                row = b; node = c / rep; head = hk * rep + c - node * rep;
-                                return c < ncol;
-                            });
+        const KeySegment s = segment_of<FMT>(A.tail, b, hk, total, base, A.sb, sp);
+        auto info = [&](int c, int& row, int& head, int& node) -> bool {
+            row = b; node = c / rep; head = hk * rep + c - node * rep;
+            return c < ncol;
+        };
+        Columns<FMT, D, NCB, decltype(info)> W(A, info, smem, c0);
+        const int first = s.t0 + W.wave;
+        if (first < s.t1) W.fetch(s, first);
+        W.load_queries();
+        W.run(s, first);
+        W.finish(smem, A.sa + sp);
     }
 }
 

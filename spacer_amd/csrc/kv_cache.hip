@@ -196,6 +196,8 @@ int spacer_check_kv_cache(const spacer_kv_cache* c, const char* who) {
     const long size = c->format == KV_BF16 ? 2 : 1;
     SP_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0 && ((c->stride_seq | c->stride_head | c->stride_pos) * size) % 16 == 0, SPACER_EINVAL,
                "%s: cache rows must start at multiples of 16 bytes", who);
+    SP_REQUIRE(c->stride_pos >= 0 && c->stride_pos * size < (1L << 26) && c->scale_stride_pos >= 0 && c->scale_stride_pos < (1L << 26), SPACER_EINVAL,
+               "%s: positions of a cache must be less than 64 MiB (scales: 2^26 floats) apart", who);
     SP_REQUIRE(c->format == KV_BF16 || (c->k_scale && c->v_scale), SPACER_EINVAL, "%s: 8-bit cache without scales", who);
     return SPACER_OK;
 }
