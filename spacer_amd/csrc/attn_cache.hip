@@ -13,12 +13,21 @@
 // Work split.  Workgroup = (prompt or sequence, kv head, column block of 16 NC, range of keys); its 4 waves take 32-key tiles in turn and never meet
 // inside the loop: the next tile's K, V and scales are requested before the current one is worked on, so 8 waves per CU keep 64 KB in flight (8 bits).
 // The waves' (O, m, l) are joined through LDS, the ranges' through fp32 records and a second small launch.
+#include <math.h>
+
 #include "kv_cache.h"
 
 namespace {
 
 constexpr int TK = 32;            // keys per wave and step
+constexpr int SOLO_MAX = 512;      // positions
 constexpr float LOG2E = 1.4426950408889634f;
+
+// n / d for 0 <= n < 2^31 by a multiplication (d is the same for a whole launch): m = floor(2^(31 + s) / d) + 1 with 2^s >= d is exact there
+struct FastDiv {
+    unsigned m, s, d;
+    __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, m) >> (s - 1)); }
+};
 
 struct AttnCacheArgs {
     const bf16_t* q;
@@ -30,6 +39,7 @@ struct AttnCacheArgs {
     int n_prompts, rows, B, N, Hq, Hkv;
     int sa, sb, cba, cbb;         // key ranges and column blocks of the prompt and of the sequence role
     int na;                       // workgroups of the prompt role (a multiple of 8)
+    FastDiv per_row, rep;         // by N * Hq / Hkv and by Hq / Hkv
     float scale;
     float* rec_o;                 // [sa + sb][B * N * Hq][D]
     float2* rec_ml;               // [sa + sb][B * N * Hq]: maximum (log2 domain) and sum
@@ -78,9 +88,11 @@ struct Tile {
     static __device__ __forceinline__ int swz(int row) { return (row / (RB >= 256 ? 1 : 256 / RB)) & (CPR - 1); }
 };
 
+// column blocks that the waves join at once: two workgroups' buffers fit a CU's 160 KB
+constexpr int join_blocks(int D, int nc) { return nc < (D == 64 ? 4 : 2) ? nc : (D == 64 ? 4 : 2); }
 constexpr int lds_bytes(int es, int D, int nc) {
     const int work = 4 * (TK * D * es + 2 * TK * 4) + (nc > 2 ? nc * (D / 32) * 64 * 16 : 0);
-    const int join = 4 * 16 * (D + 4) * 4 + 4 * 16 * 8;
+    const int join = join_blocks(D, nc) * 16 * (4 * (D + 4) * 4 + 4 * 8);
     return work > join ? work : join;
 }
 
@@ -325,55 +337,59 @@ struct Columns {
         }
     }
 
-    // joins the waves, one block of 16 columns at a time ([wave][column][D + 4 floats], [wave][column] (m, l) in LDS), and writes the record `slot` of
+    // joins the waves, RC blocks of 16 columns at a time ([wave][column][D + 4 floats], [wave][column] (m, l) in LDS), and writes the record `slot` of
     // every column, or with slot < 0 its output
     __device__ __forceinline__ void finish(char* smem, int slot) {
+        constexpr int RC = join_blocks(D, NC), JC = RC * 16, TPC = 256 / JC, PER = D / TPC;      // columns, threads per column, floats per thread
         const int tid = threadIdx.x;
         float* jo = (float*)smem;
-        float2* jm = (float2*)(smem + 4 * 16 * (D + 4) * 4);
-        constexpr int PER = D / 16;                           // floats per thread
-        const int jc = tid >> 4, jd = (tid & 15) * PER;
+        float2* jm = (float2*)(smem + 4 * JC * (D + 4) * 4);
+        const int jc = tid / TPC, jd = (tid % TPC) * 4;       // (a thread's float4 lie TPC * 4 floats apart: neighbouring threads, neighbouring banks)
         const long ncol_all = (long)A.B * A.N * A.Hq;
 #pragma unroll
-        for (int cb = 0; cb < NC; ++cb) {
+        for (int cb = 0; cb < NC; cb += RC) {
             __syncthreads();
-            float l = l_run[cb];
-            l += __shfl_xor(l, 16, 64);
-            l += __shfl_xor(l, 32, 64);
 #pragma unroll
-            for (int df = 0; df < DF; ++df)
-                *(float4*)(jo + (wave * 16 + l15) * (D + 4) + df * 16 + g * 4) = make_float4(oacc[cb][df][0], oacc[cb][df][1], oacc[cb][df][2], oacc[cb][df][3]);
-            if (g == 0) jm[wave * 16 + l15] = make_float2(m_run[cb], l);
+            for (int r = 0; r < RC; ++r) {
+                float l = l_run[cb + r];
+                l += __shfl_xor(l, 16, 64);
+                l += __shfl_xor(l, 32, 64);
+#pragma unroll
+                for (int df = 0; df < DF; ++df)
+                    *(f32x4*)(jo + (wave * JC + r * 16 + l15) * (D + 4) + df * 16 + g * 4) = oacc[cb + r][df];
+                if (g == 0) jm[wave * JC + r * 16 + l15] = make_float2(m_run[cb + r], l);
+            }
             __syncthreads();
             int row, head, node;
             if (!info(c0 + cb * 16 + jc, row, head, node)) continue;
-            float M = -INFINITY;
+            float M = -INFINITY, L = 0.f, f[4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * 16 + jc].x);
-            float L = 0.f, O[PER];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) O[i] = 0.f;
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * JC + jc].x);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float2 ml = jm[w * 16 + jc];
-                const float f = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
-                L += ml.y * f;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) O[i] += jo[(w * 16 + jc) * (D + 4) + jd + i] * f;
+                const float2 ml = jm[w * JC + jc];
+                f[w] = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+                L += ml.y * f[w];
             }
             const long col = ((long)row * A.N + node) * A.Hq + head;
-            if (slot < 0) {
-                const float inv = L == 0.f ? 0.f : 1.f / L;
+            const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-                for (int i = 0; i < PER; i += 4)
-                    *(uint2*)(A.o + col * D + jd + i) = make_uint2(pack_bf2(O[i] * inv, O[i + 1] * inv), pack_bf2(O[i + 2] * inv, O[i + 3] * inv));
-                continue;
+            for (int i = 0; i < PER / 4; ++i) {
+                const int d = jd + i * TPC * 4;
+                f32x4 O = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) O += *(const f32x4*)(jo + (w * JC + jc) * (D + 4) + d) * f[w];
+                if (slot < 0) *(uint2*)(A.o + col * D + d) = make_uint2(pack_bf2(O[0] * inv, O[1] * inv), pack_bf2(O[2] * inv, O[3] * inv));
+                else *(f32x4*)(A.rec_o + ((long)slot * ncol_all + col) * D + d) = O;
             }
-            float* ro = A.rec_o + ((long)slot * ncol_all + col) * D + jd;
-#pragma unroll
-            for (int i = 0; i < PER; i += 4) *(float4*)(ro + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
-            if ((tid & 15) == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
+            if (slot >= 0 && tid % TPC == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
         }
+    }
+    // no keys: the columns' records say so by their maximum alone
+    __device__ __forceinline__ void finish_empty(int slot) const {
+        int row, head, node;
+        if (threadIdx.x < NC * 16 && info(c0 + threadIdx.x, row, head, node))
+            A.rec_ml[(long)slot * A.B * A.N * A.Hq + ((long)row * A.N + node) * A.Hq + head] = make_float2(-INFINITY, 0.f);
     }
 };
 
@@ -399,7 +415,7 @@ __device__ __forceinline__ void rows_of(const AttnCacheArgs& A, int pr, int& r0,
 template <int FMT, int D, int NCA, int NCB>
 __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs A) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int rep = A.Hq / A.Hkv;
+    const int rep = A.rep.d;
     const bool role_a = (int)blockIdx.x < A.na;
     // column blocks of one (keys, range) go to one XCD (workgroups are dealt to the 8 XCDs in turn), next to each other: its L2 serves all but the first
     const int idx = role_a ? blockIdx.x : blockIdx.x - A.na, cbs = role_a ? A.cba : A.cbb;
@@ -414,11 +430,12 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
         const int total = min(max(A.prompt_len[pr], 0), A.prompt.cap);
         const KeySegment s = segment_of<FMT>(A.prompt, pr, hk, total, total, A.sa, sp);
         auto info = [&](int c, int& row, int& head, int& node) -> bool {
-            const int r = c / per_row, x = c - r * per_row;
-            row = r0 + r; node = x / rep; head = hk * rep + x - node * rep;
+            const int r = A.per_row(c), x = c - r * per_row;
+            row = r0 + r; node = A.rep(x); head = hk * rep + x - node * rep;
             return c < ncol;
         };
         Columns<FMT, D, NCA, decltype(info)> W(A, info, smem, c0);
+        if (s.t0 >= s.t1) return W.finish_empty(sp);
         const int first = s.t0 + W.wave;
         if (first < s.t1) W.fetch(s, first);
         W.load_queries();
@@ -432,16 +449,62 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
         const int base = min(max(A.tail_len[(long)b * A.len_stride], 0), A.tail.cap), total = min(base + A.N, A.tail.cap);
         const KeySegment s = segment_of<FMT>(A.tail, b, hk, total, base, A.sb, sp);
         auto info = [&](int c, int& row, int& head, int& node) -> bool {
-            row = b; node = c / rep; head = hk * rep + c - node * rep;
+            row = b; node = A.rep(c); head = hk * rep + c - node * rep;
             return c < ncol;
         };
         Columns<FMT, D, NCB, decltype(info)> W(A, info, smem, c0);
+        if (s.t0 >= s.t1) return W.finish_empty(A.sa + sp);
         const int first = s.t0 + W.wave;
         if (first < s.t1) W.fetch(s, first);
         W.load_queries();
         W.run(s, first);
         W.finish(smem, A.sa + sp);
     }
+}
+
+// The prompt that serves row b (-1: none), found by all lanes of a wave at once
+__device__ __forceinline__ int prompt_of_row(const AttnCacheArgs& A, int b) {
+    if (!A.row0) return min(b / A.rows, A.n_prompts - 1);
+    for (int p0 = 0; p0 < A.n_prompts; p0 += 64) {
+        const int p = p0 + (threadIdx.x & 63);
+        const bool hit = p < A.n_prompts && b >= A.row0[p] && b < A.row0[p + 1];
+        const uint64_t m = __ballot(hit);
+        if (m) return p0 + __ffsll((unsigned long long)m) - 1;
+    }
+    return -1;
+}
+
+// Short contexts: one workgroup takes the prompt's and the sequence's keys of its columns and writes their output itself.
+template <int FMT, int D, int NC>
+__global__ __launch_bounds__(256, 2) void attn_cache_solo_kernel(const AttnCacheArgs A) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int rep = A.rep.d, cb = blockIdx.x % A.cbb, hk = (blockIdx.x / A.cbb) % A.Hkv, b = blockIdx.x / (A.cbb * A.Hkv);
+    const int ncol = A.N * rep;
+    auto info = [&](int c, int& row, int& head, int& node) -> bool {
+        row = b; node = A.rep(c); head = hk * rep + c - node * rep;
+        return c < ncol;
+    };
+    Columns<FMT, D, NC, decltype(info)> W(A, info, smem, cb * 16 * NC);
+    W.load_queries();
+    int nt = 0;
+    if (A.n_prompts) {
+        const int pr = __builtin_amdgcn_readfirstlane(prompt_of_row(A, b));
+        if (pr >= 0) {
+            const int total = min(max(A.prompt_len[pr], 0), A.prompt.cap);
+            const KeySegment s = segment_of<FMT>(A.prompt, pr, hk, total, total, 1, 0);
+            if (W.wave < s.t1) W.fetch(s, W.wave);
+            W.run(s, W.wave);
+            nt = s.t1;
+        }
+    }
+    if (A.tail.k) {
+        const int base = min(max(A.tail_len[(long)b * A.len_stride], 0), A.tail.cap), total = min(base + A.N, A.tail.cap);
+        const KeySegment s = segment_of<FMT>(A.tail, b, hk, total, base, 1, 0);
+        const int first = (W.wave - nt) & 3;              // the waves go on in turn
+        if (first < s.t1) W.fetch(s, first);
+        W.run(s, first);
+    }
+    W.finish(smem, -1);
 }
 
 // o = the softmax-weighted join of a column's records; D / 4 lanes per column.  A sequence that no prompt owns has no prompt records.
@@ -458,53 +521,94 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(const AttnCacheArg
         if (b < lo || b >= hi) first = A.sa;
     }
     const int ns = A.sa + A.sb;
-    float M = -INFINITY;
-#pragma unroll 4
-    for (int s = first; s < ns; ++s) M = fmaxf(M, A.rec_ml[s * ncol + col].x);
-    float L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = first; s < ns; ++s) {
-        const float2 ml = A.rec_ml[s * ncol + col];
-        const float4 x = *(const float4*)(A.rec_o + (s * ncol + col) * D + d);
-        const float f = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
-        L += ml.y * f;
-        O[0] += x.x * f; O[1] += x.y * f; O[2] += x.z * f; O[3] += x.w * f;
+    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = first; s0 < ns; s0 += 8) {              // eight records per memory round trip
+        float2 ml[8];
+        float4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const long at = min(s0 + i, ns - 1) * ncol + col;
+            ml[i] = A.rec_ml[at];
+            x[i] = *(const float4*)(A.rec_o + at * D + d);
+        }
+        float m = M;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, ml[i].x);
+        const float f0 = M == m ? 1.f : __builtin_amdgcn_exp2f(M - m);
+        M = m;
+        L *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[e] *= f0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (s0 + i >= ns || ml[i].x == -INFINITY) continue;
+            const float f = ml[i].x == M ? 1.f : __builtin_amdgcn_exp2f(ml[i].x - M);
+            L += ml[i].y * f;
+            O[0] += x[i].x * f; O[1] += x[i].y * f; O[2] += x[i].z * f; O[3] += x[i].w * f;
+        }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     *(uint2*)(A.o + col * D + d) = make_uint2(pack_bf2(O[0] * inv, O[1] * inv), pack_bf2(O[2] * inv, O[3] * inv));
 }
 
 struct AttnPlan {
-    int nca, ncb, cba, cbb, sa, sb;
+    int solo, nca, ncb, cba, cbb, sa, sb;
     long cols;
 };
 
-// Column blocks: as wide as the columns need, up to 64 (a wave's fp32 O of 64 x 128 is 128 registers).  Key ranges: the launch's keys x column
-// blocks spread over 512 workgroups (two per CU, all resident), at least 256 keys (two tiles per wave) each; the capacities stand for the lengths,
-// which only the device knows.
+// Column blocks: as wide as the columns need, up to 64 (a wave's fp32 O of 64 x 128 is 128 registers).
+// Key ranges: the pair (sa, sb) whose estimated time is least: 512 workgroups run at once (two per CU); one costs its 32-key tiles per wave, a wide
+// tile about twice a narrow one, and some 4 tiles for its start and its end.  The capacities stand for the lengths, which only the device knows; half of
+// the tail's, which fills up while a rollout runs.
+// Solo: contexts of up to 512 positions (16 tiles, 4 per wave) in one launch without records.
 AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
     const spacer_kv_cache* c = prompt ? prompt : tail;
     const int rep = Hq / c->kv_heads;
-    const long ca = prompt ? (long)rows * N * rep : 0, cb = tail ? (long)N * rep : 0;
+    const long ca = prompt ? (long)rows * N * rep : 0, cb = (long)N * rep;
     AttnPlan p;
-    const long most = ca > cb ? ca : cb;
+    p.cols = (long)B * N * Hq;
+    p.solo = (long)(prompt ? prompt->capacity : 0) + (tail ? tail->capacity : 0) <= SOLO_MAX;
+    if (p.solo) {
+        p.nca = p.ncb = cb <= 16 ? 1 : cb <= 32 ? 2 : 4;
+        p.cba = 0; p.cbb = cdiv(cb, 16 * p.ncb);
+        p.sa = p.sb = 0;
+        return p;
+    }
+    const long cbt = tail ? cb : 0, most = ca > cbt ? ca : cbt;
     if (most <= 16) p.nca = p.ncb = 1;
-    else if (cb <= 16) { p.nca = 4; p.ncb = 1; }
+    else if (cbt <= 16) { p.nca = 4; p.ncb = 1; }
     else if (most <= 32) p.nca = p.ncb = 2;
     else p.nca = p.ncb = 4;
     p.cba = prompt ? cdiv(ca, 16 * p.nca) : 0;
-    p.cbb = tail ? cdiv(cb, 16 * p.ncb) : 0;
+    p.cbb = tail ? cdiv(cbt, 16 * p.ncb) : 0;
     const double ja = prompt ? (double)prompt->n_seq * c->kv_heads * p.cba : 0, jb = tail ? (double)B * c->kv_heads * p.cbb : 0;
-    double keys = (prompt ? ja * prompt->capacity : 0) + (tail ? jb * tail->capacity : 0);
-    keys /= 512;
-    const long range = keys < 256 ? 256 : keys > 1e9 ? 1000000000L : (long)keys + 1;
-    p.sa = prompt ? cdiv(prompt->capacity, range) : 0;
-    p.sb = tail ? cdiv(tail->capacity, range) : 0;
-    p.cols = (long)B * N * Hq;
+    const double ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
+    const double wa = 0.5 + 0.5 * p.nca, wb = 0.5 + 0.5 * p.ncb, start = 4.0;
+    double best = 1e300;
+    p.sa = prompt ? 1 : 0; p.sb = tail ? 1 : 0;
+    for (int sb = tail ? 1 : 0; sb <= (tail ? 4 : 0); ++sb) {
+        if (sb > 1 && tb / sb < 2) break;
+        for (int sa = prompt ? 1 : 0; sa <= (prompt ? 64 : 0); sa += sa < 16 ? 1 : 4) {
+            if (sa > 1 && ta / sa < 1) break;
+            const double a = sa ? start + ceil(ta / sa) * wa : 0, b = sb ? start + ceil(tb / sb) * wb : 0, longest = a > b ? a : b;
+            const double blocks = ja * sa + jb * sb, work = (ja * sa * a + jb * sb * b) / 512;
+            double t = work > longest ? work : longest;
+            if (blocks > 512) t += 0.25 * (a > b && b > 0 ? b : a > 0 ? a : b);          // a second round rarely ends together
+            t += 0.15 * (sa + sb);                                                       // records to write and join
+            if (t < best - 1e-9) { best = t; p.sa = sa; p.sb = sb; }
+        }
+    }
     return p;
 }
 
 }  // namespace
+
+static FastDiv fast_div(unsigned d) {
+    FastDiv f = {0, 0, d};
+    while ((1u << f.s) < d) ++f.s;
+    f.m = (unsigned)((1ull << (31 + f.s)) / d) + 1;
+    return f;
+}
 
 static int check_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
     SP_REQUIRE(prompt || tail, SPACER_EINVAL, "attn_cache: no cache");
@@ -543,7 +647,7 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
     SP_REQUIRE(!tail || tail_len, SPACER_EINVAL, "attn_cache: tail_len required");
     const AttnPlan p = plan_attn(prompt, tail, rows, B, N, Hq);
     const long need = (p.sa + p.sb) * p.cols * (D + 2) * 4L;
-    SP_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, SPACER_ENOMEM, "attn_cache: workspace of %ld bytes, %ld needed",
+    SP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), SPACER_ENOMEM, "attn_cache: workspace of %ld bytes, %ld needed",
                workspace ? workspace_bytes : 0L, need);
     AttnCacheArgs A = {};
     A.q = (const bf16_t*)q; A.q_ld = q_ld;
@@ -554,16 +658,45 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
     A.rows = rows; A.B = B; A.N = N; A.Hq = Hq; A.Hkv = Hkv;
     A.sa = p.sa; A.sb = p.sb; A.cba = p.cba; A.cbb = p.cbb;
     A.scale = scale;
+    A.rep = fast_div(Hq / Hkv);
+    A.per_row = fast_div(N * (Hq / Hkv));
     A.rec_o = (float*)workspace;
     A.rec_ml = (float2*)(A.rec_o + (p.sa + p.sb) * p.cols * D);
     A.o = (bf16_t*)o;
+    hipStream_t s = (hipStream_t)stream;
+    if (p.solo) {
+        const long n = (long)B * Hkv * p.cbb;
+        SP_REQUIRE(n <= 0x7fffffffL, SPACER_EINVAL, "attn_cache: too many workgroups");
+#define LAUNCH(F, DD, NC)                                                                                                                           \
+    do {                                                                                                                                            \
+        constexpr int lds = lds_bytes(kv_size<F>(), DD, NC);                                                                                         \
+        static const hipError_t once = hipFuncSetAttribute((const void*)attn_cache_solo_kernel<F, DD, NC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
+        (void)once;                                                                                                                                 \
+        hipLaunchKernelGGL((attn_cache_solo_kernel<F, DD, NC>), dim3((unsigned)n), dim3(256), lds, s, A);                                            \
+    } while (0)
+#define CALL(F, DD)                                                                                                                                 \
+    do {                                                                                                                                            \
+        if (p.ncb == 1) LAUNCH(F, DD, 1);                                                                                                           \
+        else if (p.ncb == 2) LAUNCH(F, DD, 2);                                                                                                      \
+        else LAUNCH(F, DD, 4);                                                                                                                      \
+    } while (0)
+        KV_DISPATCH(c, CALL);
+#undef CALL
+#undef LAUNCH
+        SP_CHECK_LAUNCH();
+        return SPACER_OK;
+    }
     const long ja = prompt ? (long)prompt->n_seq * Hkv * p.sa : 0, jb = tail ? (long)B * Hkv * p.sb : 0;
     const long na = (ja + 7) / 8 * 8 * p.cba, nb = (jb + 7) / 8 * 8 * p.cbb;
     SP_REQUIRE(na + nb <= 0x7fffffffL, SPACER_EINVAL, "attn_cache: too many workgroups");
     A.na = (int)na;
-    hipStream_t s = (hipStream_t)stream;
 #define LAUNCH(F, DD, NA, NB)                                                                                                                       \
-    hipLaunchKernelGGL((attn_cache_kernel<F, DD, NA, NB>), dim3((unsigned)(na + nb)), dim3(256), lds_bytes(kv_size<F>(), DD, NA > NB ? NA : NB), s, A)
+    do {                                                                                                                                            \
+        constexpr int lds = lds_bytes(kv_size<F>(), DD, NA > NB ? NA : NB);                                                                          \
+        static const hipError_t once = hipFuncSetAttribute((const void*)attn_cache_kernel<F, DD, NA, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
+        (void)once;                                                                                                                                 \
+        hipLaunchKernelGGL((attn_cache_kernel<F, DD, NA, NB>), dim3((unsigned)(na + nb)), dim3(256), lds, s, A);                                     \
+    } while (0)
 #define CALL(F, DD)                                                                                                                                 \
     do {                                                                                                                                            \
         if (p.nca == 1) LAUNCH(F, DD, 1, 1);                                                                                                        \

@@ -26,46 +26,58 @@ __device__ __forceinline__ void store_row(char* dst, float* scale, const uint4 x
     if (lane_in_row == 0) *scale = r.scale;
 }
 
-// APPEND == false: row (slot, head) takes source row rows[slot] (below 0, or >= n_src: the slot stays as it is)
-// APPEND == true : row (b N + i, head) goes to position len[b] + i of sequence b (outside the cache: dropped)
+// Rows of a pass: sequence (blockIdx.x / chunks, a scalar), then row = position * Hkv + head inside it (32 bits), so that the heads of a token,
+// side by side in the source, fall to one wave.  A lane holds a piece of RU rows at once: their loads are in flight together.
+constexpr int RU = 1;
+template <int D> constexpr int rows_per_step() { return 4 * (512 / D) * RU; }      // rows that a workgroup takes at once
+
+// APPEND == false: slot (sequence, position) takes source row rows[slot] (below 0, or >= n_src: the slot stays as it is)
+// APPEND == true : source row sequence * N + i goes to position len[sequence] + i (outside the cache: dropped)
 template <int FMT, int D, bool APPEND>
 __global__ __launch_bounds__(256) void kv_store_kernel(const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, long ld, int n_src,
                                                        const int* __restrict__ rows, const int* __restrict__ len, int len_stride, int N,
-                                                       KvView c, int Hkv, long total) {
+                                                       KvView c, unsigned Hkv, unsigned chunks, unsigned steps) {
     constexpr int LPR = D / 8, RPW = 64 / LPR;       // lanes per row, rows per wave
     const int lane = threadIdx.x & 63, lr = lane % LPR;
-    const long nw = (long)gridDim.x * 4;
-    // (row ids of one wave are consecutive: the heads of a token lie side by side in the source)
-    for (long r0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW; r0 < total; r0 += nw * RPW) {
-        const long rid = r0 + lane / LPR;
-        long src = -1;
-        int seq = 0, pos = 0, h = 0;
-        if (rid < total) {
-            h = (int)(rid % Hkv);
-            const long slot = rid / Hkv;
-            if (APPEND) {
-                seq = (int)(slot / N);
-                const long p = (long)len[(long)seq * len_stride] + slot % N;
-                src = (p >= 0 && p < c.cap) ? slot : -1;
-                pos = (int)p;
-            } else {
-                seq = (int)(slot / c.cap);
-                pos = (int)(slot % c.cap);
-                src = rows[slot];
-                if (src >= n_src) src = -1;
+    const unsigned seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const unsigned total = (unsigned)(APPEND ? N : c.cap) * Hkv;
+    const long first = APPEND ? (long)len[(long)seq * len_stride] : 0;
+    for (unsigned step = 0; step < steps; ++step) {
+        const unsigned r0 = (chunk * steps + step) * rows_per_step<D>() + (threadIdx.x >> 6) * (RPW * RU) + lane / LPR;
+        int pos[RU], h[RU];
+        long src[RU];
+#pragma unroll
+        for (int u = 0; u < RU; ++u) {
+            const unsigned r = r0 + u * RPW, i = r / Hkv;
+            h[u] = (int)(r - i * Hkv);
+            src[u] = -1;
+            if (r < total) {
+                if (APPEND) {
+                    const long p = first + i;
+                    pos[u] = (int)p;
+                    if (p >= 0 && p < c.cap) src[u] = (long)seq * N + i;
+                } else {
+                    pos[u] = (int)i;
+                    src[u] = rows[(long)seq * c.cap + i];
+                    if (src[u] >= n_src) src[u] = -1;
+                }
             }
         }
-        const bool live = src >= 0;
-        uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
-        if (live) {
-            xk = *(const uint4*)(k + src * ld + h * D + lr * 8);
-            xv = *(const uint4*)(v + src * ld + h * D + lr * 8);
-        }
-        if (!live) continue;                         // (whole rows drop out: the lanes of a row stay together)
-        const long at = (seq * c.s_seq + h * c.s_head + pos * c.s_pos) * kv_size<FMT>();
-        const long sat = seq * c.c_seq + h * c.c_head + pos * c.c_pos;
-        store_row<FMT, D>(c.k + at, c.ks + sat, xk, lr);
-        store_row<FMT, D>(c.v + at, c.vs + sat, xv, lr);
+        uint4 xk[RU], xv[RU];
+#pragma unroll
+        for (int u = 0; u < RU; ++u)
+            if (src[u] >= 0) {                           // (the lanes of a row drop out together)
+                xk[u] = *(const uint4*)(k + src[u] * ld + h[u] * D + lr * 8);
+                xv[u] = *(const uint4*)(v + src[u] * ld + h[u] * D + lr * 8);
+            }
+#pragma unroll
+        for (int u = 0; u < RU; ++u)
+            if (src[u] >= 0) {
+                const long at = (seq * c.s_seq + h[u] * c.s_head + pos[u] * c.s_pos) * kv_size<FMT>();
+                const long sat = seq * c.c_seq + h[u] * c.c_head + pos[u] * c.c_pos;
+                store_row<FMT, D>(c.k + at, c.ks + sat, xk[u], lr);
+                store_row<FMT, D>(c.v + at, c.vs + sat, xv[u], lr);
+            }
     }
 }
 
@@ -94,34 +106,42 @@ __device__ __forceinline__ void values8(const char* p, float s, float (&f)[8]) {
     for (int i = 0; i < 8; ++i) f[i] *= s;
 }
 
+constexpr int RD = 2;
 template <int FMT, int D, bool F32>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvView c, const int* __restrict__ len, void* __restrict__ ko, void* __restrict__ vo,
-                                                      int Hkv, long total) {
+                                                      unsigned Hkv, unsigned chunks) {
     constexpr int LPR = D / 8, RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, lr = lane % LPR;
-    const long nw = (long)gridDim.x * 4;
-    for (long r0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW; r0 < total; r0 += nw * RPW) {
-        const long rid = r0 + lane / LPR;
-        if (rid >= total) continue;
-        const int h = (int)(rid % Hkv);
-        const long slot = rid / Hkv;
-        const int seq = (int)(slot / c.cap), pos = (int)(slot % c.cap);
-        float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (!len || pos < len[seq]) {
-            const long at = (seq * c.s_seq + h * c.s_head + pos * c.s_pos + lr * 8) * kv_size<FMT>();
-            const long sat = seq * c.c_seq + h * c.c_head + pos * c.c_pos;
+    const unsigned seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const unsigned total = (unsigned)c.cap * Hkv;
+    const unsigned r0 = chunk * (4 * RPW * RD) + (threadIdx.x >> 6) * (RPW * RD) + lane / LPR;
+    const int n = len ? len[seq] : c.cap;
+    float a[RD][8], b[RD][8];
+#pragma unroll
+    for (int u = 0; u < RD; ++u) {
+        const unsigned r = r0 + u * RPW, i = r / Hkv, h = r - i * Hkv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[u][e] = b[u][e] = 0.f;
+        if (r < total && (int)i < n) {
+            const long at = (seq * c.s_seq + h * c.s_head + i * c.s_pos + lr * 8) * kv_size<FMT>();
+            const long sat = seq * c.c_seq + h * c.c_head + i * c.c_pos;
             const float sk = FMT == KV_BF16 ? 1.f : c.ks[sat], sv = FMT == KV_BF16 ? 1.f : c.vs[sat];
-            values8<FMT>(c.k + at, sk, a);
-            values8<FMT>(c.v + at, sv, b);
+            values8<FMT>(c.k + at, sk, a[u]);
+            values8<FMT>(c.v + at, sv, b[u]);
         }
-        const long o = rid * D + lr * 8;
+    }
+#pragma unroll
+    for (int u = 0; u < RD; ++u) {
+        const unsigned r = r0 + u * RPW;
+        if (r >= total) continue;
+        const long o = ((long)seq * total + r) * D + lr * 8;
         if (F32) {
             float *kp = (float*)ko + o, *vp = (float*)vo + o;
-            *(float4*)kp = make_float4(a[0], a[1], a[2], a[3]); *(float4*)(kp + 4) = make_float4(a[4], a[5], a[6], a[7]);
-            *(float4*)vp = make_float4(b[0], b[1], b[2], b[3]); *(float4*)(vp + 4) = make_float4(b[4], b[5], b[6], b[7]);
+            *(float4*)kp = make_float4(a[u][0], a[u][1], a[u][2], a[u][3]); *(float4*)(kp + 4) = make_float4(a[u][4], a[u][5], a[u][6], a[u][7]);
+            *(float4*)vp = make_float4(b[u][0], b[u][1], b[u][2], b[u][3]); *(float4*)(vp + 4) = make_float4(b[u][4], b[u][5], b[u][6], b[u][7]);
         } else {
-            *(uint4*)((bf16_t*)ko + o) = make_uint4(pack_bf2(a[0], a[1]), pack_bf2(a[2], a[3]), pack_bf2(a[4], a[5]), pack_bf2(a[6], a[7]));
-            *(uint4*)((bf16_t*)vo + o) = make_uint4(pack_bf2(b[0], b[1]), pack_bf2(b[2], b[3]), pack_bf2(b[4], b[5]), pack_bf2(b[6], b[7]));
+            *(uint4*)((bf16_t*)ko + o) = make_uint4(pack_bf2(a[u][0], a[u][1]), pack_bf2(a[u][2], a[u][3]), pack_bf2(a[u][4], a[u][5]), pack_bf2(a[u][6], a[u][7]));
+            *(uint4*)((bf16_t*)vo + o) = make_uint4(pack_bf2(b[u][0], b[u][1]), pack_bf2(b[u][2], b[u][3]), pack_bf2(b[u][4], b[u][5]), pack_bf2(b[u][6], b[u][7]));
         }
     }
 }
@@ -207,8 +227,14 @@ KvView spacer_kv_view(const spacer_kv_cache* c) {
                   c->scale_stride_head, c->scale_stride_pos, c->n_seq, c->capacity};
 }
 
-// workgroups of a row pass: 4 waves each, enough to cover the rows, at most 16 per CU (the loop strides over the rest)
-static int row_grid(long total, int D) { return (int)min(cdiv(total, 4 * (512 / D)), 256 * 16); }
+// Workgroups of a sequence's `rows` rows, `per` each, or 0 where the launch would not fit
+static unsigned row_chunks(long n_seq, long rows, int per) {
+    const long chunks = (rows + per - 1) / per;
+    return rows < 0x7fffffffL - 4096 && n_seq * chunks <= 0x7fffffffL ? (unsigned)chunks : 0u;
+}
+// A workgroup takes 4 steps where that still leaves two workgroups per CU: the scales of neighbouring positions (4 bytes each) then leave one
+// workgroup, i.e. one XCD's L2, as whole lines.
+static unsigned store_steps(long n_seq, long rows, int D) { return 1; }
 
 static int check_source(const void* k, const void* v, long ld, const char* who) {
     SP_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ld % 8 == 0, SPACER_EINVAL, "%s: source rows must start at multiples of 16 bytes", who);
@@ -220,10 +246,12 @@ extern "C" int spacer_kv_write(const spacer_kv_cache* c, const void* k, const vo
     SP_REQUIRE(n_src >= 0 && rows, SPACER_EINVAL, "kv_write: rows required, n_src >= 0");
     if (n_src == 0) return SPACER_OK;
     if (int rc = check_source(k, v, ld, "kv_write")) return rc;
-    const long total = (long)c->n_seq * c->capacity * c->kv_heads;
+    const long per_seq = (long)c->capacity * c->kv_heads;
+    const unsigned steps = store_steps(c->n_seq, per_seq, c->head_dim), chunks = row_chunks(c->n_seq, per_seq, steps * 4 * (512 / c->head_dim) * RU);
+    SP_REQUIRE(chunks, SPACER_EINVAL, "kv_write: cache too large");
 #define CALL(F, D)                                                                                                                                   \
-    hipLaunchKernelGGL((kv_store_kernel<F, D, false>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
-                       ld, n_src, rows, (const int*)nullptr, 0, 1, spacer_kv_view(c), c->kv_heads, total)
+    hipLaunchKernelGGL((kv_store_kernel<F, D, false>), dim3(c->n_seq * chunks), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
+                       ld, n_src, rows, (const int*)nullptr, 0, 1, spacer_kv_view(c), c->kv_heads, chunks, steps)
     KV_DISPATCH(c, CALL);
 #undef CALL
     SP_CHECK_LAUNCH();
@@ -236,11 +264,12 @@ extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const v
     SP_REQUIRE(N >= 0 && len, SPACER_EINVAL, "kv_append: lengths required, N >= 0");
     if (N == 0) return SPACER_OK;
     if (int rc = check_source(k, v, ld, "kv_append")) return rc;
-    SP_REQUIRE((long)c->n_seq * N <= 0x7fffffffL, SPACER_EINVAL, "kv_append: %d sequences x %d tokens are too many", c->n_seq, N);
-    const long total = (long)c->n_seq * N * c->kv_heads;
+    const long per_seq = (long)N * c->kv_heads;
+    const unsigned steps = store_steps(c->n_seq, per_seq, c->head_dim), chunks = row_chunks(c->n_seq, per_seq, steps * 4 * (512 / c->head_dim) * RU);
+    SP_REQUIRE(chunks && (long)c->n_seq * N <= 0x7fffffffL, SPACER_EINVAL, "kv_append: %d sequences x %d tokens are too many", c->n_seq, N);
 #define CALL(F, D)                                                                                                                                  \
-    hipLaunchKernelGGL((kv_store_kernel<F, D, true>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
-                       ld, c->n_seq * N, (const int*)nullptr, len, len_per_seq ? 1 : 0, N, spacer_kv_view(c), c->kv_heads, total)
+    hipLaunchKernelGGL((kv_store_kernel<F, D, true>), dim3(c->n_seq * chunks), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
+                       ld, c->n_seq * N, (const int*)nullptr, len, len_per_seq ? 1 : 0, N, spacer_kv_view(c), c->kv_heads, chunks, steps)
     KV_DISPATCH(c, CALL);
 #undef CALL
     SP_CHECK_LAUNCH();
@@ -250,15 +279,16 @@ extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const v
 extern "C" int spacer_kv_read(const spacer_kv_cache* c, const int* len, void* k_out, void* v_out, int out_f32, spacer_stream_t stream) {
     if (int rc = spacer_check_kv_cache(c, "kv_read")) return rc;
     SP_REQUIRE(k_out && v_out && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, SPACER_EINVAL, "kv_read: outputs must be 16-byte aligned");
-    const long total = (long)c->n_seq * c->capacity * c->kv_heads;
+    const unsigned chunks = row_chunks(c->n_seq, (long)c->capacity * c->kv_heads, 4 * (512 / c->head_dim) * RD);
+    SP_REQUIRE(chunks, SPACER_EINVAL, "kv_read: cache too large");
 #define CALL(F, D)                                                                                                                                   \
     do {                                                                                                                                             \
         if (out_f32)                                                                                                                                 \
-            hipLaunchKernelGGL((kv_read_kernel<F, D, true>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, spacer_kv_view(c), len, k_out, \
-                               v_out, c->kv_heads, total);                                                                                           \
+            hipLaunchKernelGGL((kv_read_kernel<F, D, true>), dim3(c->n_seq * chunks), dim3(256), 0, (hipStream_t)stream, spacer_kv_view(c), len, k_out, \
+                               v_out, c->kv_heads, chunks);                                                                                           \
         else                                                                                                                                         \
-            hipLaunchKernelGGL((kv_read_kernel<F, D, false>), dim3(row_grid(total, D)), dim3(256), 0, (hipStream_t)stream, spacer_kv_view(c), len, k_out, \
-                               v_out, c->kv_heads, total);                                                                                           \
+            hipLaunchKernelGGL((kv_read_kernel<F, D, false>), dim3(c->n_seq * chunks), dim3(256), 0, (hipStream_t)stream, spacer_kv_view(c), len, k_out, \
+                               v_out, c->kv_heads, chunks);                                                                                           \
     } while (0)
     KV_DISPATCH(c, CALL);
 #undef CALL

@@ -18,12 +18,11 @@ struct LogitArgs {
     int n_masks;
     float rep, freq, pres;
     const float *rep_dev, *freq_dev, *pres_dev, *bias;
-    int in_place;
 };
 
 constexpr int LU = 4;              // float4 groups per thread
 
-template <bool VEC>
+template <bool VEC, bool IN_PLACE>
 __global__ __launch_bounds__(256) void process_logits_kernel(const LogitArgs A) {
     const int b = blockIdx.y;
     const float* in = A.in + (long)b * A.ld;
@@ -31,52 +30,65 @@ __global__ __launch_bounds__(256) void process_logits_kernel(const LogitArgs A) 
     const float* bias = A.bias ? A.bias + (long)b * A.ld_bias : nullptr;
     const uint8_t* seen = A.seen ? (const uint8_t*)(A.seen + (long)b * A.words) : nullptr;
     const int* counts = A.counts ? A.counts + (long)b * A.vocab : nullptr;
+    const int base = blockIdx.x * (256 * 4 * LU) + threadIdx.x * 4;
+    // out of place every logit is read: first of all, beside the bits
+    float4 x[LU], bb[LU];
+    uint32_t s4[LU], a4[LU];
+    if (VEC && !IN_PLACE) {
+#pragma unroll
+        for (int u = 0; u < LU; ++u) {
+            const int v = base + u * 1024;
+            if (v + 4 <= A.vocab) x[u] = *(const float4*)(in + v);
+        }
+    }
     const uint8_t* mask = nullptr;
     if (A.allowed) {
         const int m = A.allowed_row ? A.allowed_row[b] : A.n_masks == 1 ? 0 : b;
         if (m >= 0 && m < A.n_masks) mask = (const uint8_t*)(A.allowed + (long)m * A.words);
     }
-    const float r = A.rep_dev ? A.rep_dev[b] : A.rep, f = A.freq_dev ? A.freq_dev[b] : A.freq, pr = A.pres_dev ? A.pres_dev[b] : A.pres;
-    auto penal = [&](float x, int v) -> float {            // token v, seen: everything but the mask
-        double d = x;
-        d = d > 0.0 ? d / (double)r : d * (double)r;
-        if (counts) {
-            const int n = counts[v];
-            d -= (double)f * n + (n > 0 ? (double)pr : 0.0);
-        }
-        if (bias) d += (double)bias[v];
-        return (float)d;
-    };
-    const int base = blockIdx.x * (256 * 4 * LU) + threadIdx.x * 4;
-    uint32_t s4[LU], a4[LU];
 #pragma unroll
     for (int u = 0; u < LU; ++u) {
         const int v = base + u * 1024;
         s4[u] = 0; a4[u] = 15;
+        bb[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (v < A.vocab) {                                 // (bits of a byte past the vocabulary belong to the row's last word: readable)
             if (seen) s4[u] = (seen[v >> 3] >> (v & 4)) & 15u;
             if (mask) a4[u] = (mask[v >> 3] >> (v & 4)) & 15u;
+            if (VEC && bias && v + 4 <= A.vocab) bb[u] = *(const float4*)(bias + v);
         }
     }
-    float4 x[LU], bb[LU];
-    bool full[LU], need[LU];
+    const double r = A.rep_dev ? A.rep_dev[b] : A.rep, inv_r = 1.0 / r;
+    const double f = A.freq_dev ? A.freq_dev[b] : A.freq, pr = A.pres_dev ? A.pres_dev[b] : A.pres;
+    auto penal = [&](float xf, int n, float be) -> float { // a seen token with n occurrences in the completion
+        double d = xf;
+        d *= d > 0.0 ? inv_r : r;
+        if (counts) d -= f * n + (n > 0 ? pr : 0.0);
+        return (float)(bias ? d + (double)be : d);
+    };
+    if (VEC && IN_PLACE) {
 #pragma unroll
-    for (int u = 0; u < LU; ++u) {
-        const int v = base + u * 1024;
-        full[u] = VEC && v + 4 <= A.vocab;
-        need[u] = v < A.vocab && (!A.in_place || bias || (s4[u] & a4[u]));
-        bb[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (full[u] && need[u]) {
-            x[u] = *(const float4*)(in + v);
-            if (bias) bb[u] = *(const float4*)(bias + v);
+        for (int u = 0; u < LU; ++u) {
+            const int v = base + u * 1024;
+            if (v + 4 <= A.vocab && (bias || (s4[u] & a4[u]))) x[u] = *(const float4*)(in + v);
         }
+    }
+    int n4[LU][4];
+    if (VEC && counts) {                                   // the counts behind all set bits, in flight together
+#pragma unroll
+        for (int u = 0; u < LU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = base + u * 1024 + e;
+                n4[u][e] = 0;
+                if (((s4[u] & a4[u]) >> e) & 1 && base + u * 1024 + 4 <= A.vocab) n4[u][e] = counts[v];
+            }
     }
 #pragma unroll
     for (int u = 0; u < LU; ++u) {
         const int v = base + u * 1024;
         if (v >= A.vocab) continue;
-        if (full[u]) {
-            if (!need[u]) {                                // in place: nothing to compute, perhaps tokens to forbid
+        if (VEC && v + 4 <= A.vocab) {
+            if (IN_PLACE && !bias && !(s4[u] & a4[u])) {   // nothing to compute, perhaps tokens to forbid
                 if (a4[u] == 15u) continue;
                 if (a4[u] == 0u) { *(float4*)(out + v) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); continue; }
 #pragma unroll
@@ -86,35 +98,69 @@ __global__ __launch_bounds__(256) void process_logits_kernel(const LogitArgs A) 
             }
             float y[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
             const float be[4] = {bb[u].x, bb[u].y, bb[u].z, bb[u].w};
+            if (s4[u] & a4[u]) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[e] = ((s4[u] >> e) & 1) ? penal(y[e], v + e) : bias ? y[e] + be[e] : y[e];
-                if (!((a4[u] >> e) & 1)) y[e] = -INFINITY;
+                for (int e = 0; e < 4; ++e) {
+                    const float z = penal(y[e], counts ? n4[u][e] : 0, be[e]);
+                    y[e] = ((s4[u] >> e) & 1) ? z : bias ? y[e] + be[e] : y[e];
+                }
+            } else if (bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += be[e];
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!((a4[u] >> e) & 1)) y[e] = -INFINITY;
             *(float4*)(out + v) = make_float4(y[0], y[1], y[2], y[3]);
         } else {
             for (int e = 0; e < 4 && v + e < A.vocab; ++e) {
                 const bool sn = (s4[u] >> e) & 1, al = (a4[u] >> e) & 1;
+                const float be = bias ? bias[v + e] : 0.f;
                 if (!al) out[v + e] = -INFINITY;
-                else if (sn) out[v + e] = penal(in[v + e], v + e);
-                else if (bias) out[v + e] = in[v + e] + bias[v + e];
-                else if (!A.in_place) out[v + e] = in[v + e];
+                else if (sn) out[v + e] = penal(in[v + e], counts ? counts[v + e] : 0, be);
+                else if (bias) out[v + e] = in[v + e] + be;
+                else if (!IN_PLACE) out[v + e] = in[v + e];
             }
         }
     }
 }
 
-// One thread per id.  A prompt repeats its placeholder token thousands of times: the bit is read before the atomic that would set it.
+// Few ids: one thread each.  (A workgroup of the form below would clear and flush a whole bit map for them.)
 __global__ __launch_bounds__(256) void token_history_kernel(int* __restrict__ seen, int* __restrict__ counts, int vocab, int words,
                                                             const int64_t* __restrict__ ids, long ld, int n, const int* __restrict__ len) {
     const int b = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
     if (i >= n || (len && i >= len[b])) return;
     const int64_t v = ids[(long)b * ld + i];
     if (v < 0 || v >= vocab) return;
-    int* w = seen + (long)b * words + (v >> 5);
-    const int bit = (int)(1u << (v & 31));
-    if (!(__hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit)) atomicOr(w, bit);
+    atomicOr(seen + (long)b * words + (v >> 5), (int)(1u << (v & 31)));
     if (counts) atomicAdd(counts + (long)b * vocab + v, 1);
+}
+
+// Many ids: one workgroup per row collects the bits in LDS (a prompt repeats its placeholder token thousands of times, and a set bit costs an LDS
+// atomic there instead of one in memory) and owns the row's words, so that they are merged without atomics.
+__global__ __launch_bounds__(1024) void token_history_row_kernel(int* __restrict__ seen, int* __restrict__ counts, int vocab, int words,
+                                                                 const int64_t* __restrict__ ids, long ld, int n, const int* __restrict__ len) {
+    extern __shared__ int bits[];
+    const int b = blockIdx.x;
+    const int m = len ? min(n, len[b]) : n;
+    for (int i = threadIdx.x; i < words; i += 1024) bits[i] = 0;
+    __syncthreads();
+    for (int i0 = threadIdx.x; i0 < m; i0 += 4 * 1024) {
+        int64_t v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = i0 + u * 1024 < m ? ids[(long)b * ld + i0 + u * 1024] : -1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (v[u] < 0 || v[u] >= vocab) continue;
+            const int bit = (int)(1u << (v[u] & 31));
+            if (!(bits[v[u] >> 5] & bit)) atomicOr(bits + (v[u] >> 5), bit);
+            if (counts) __hip_atomic_fetch_add(counts + (long)b * vocab + v[u], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+    }
+    __syncthreads();
+    int* w = seen + (long)b * words;
+    for (int i = threadIdx.x; i < words; i += 1024)
+        if (bits[i]) w[i] |= bits[i];
 }
 
 }  // namespace
@@ -124,7 +170,10 @@ extern "C" int spacer_token_history_add(int* seen, int* counts, int B, int vocab
     if (B == 0 || n == 0) return SPACER_OK;
     SP_REQUIRE(seen && ids, SPACER_EINVAL, "token_history_add: seen and ids required");
     SP_REQUIRE(B <= 65535, SPACER_EINVAL, "token_history_add: %d rows (at most 65535)", B);
-    hipLaunchKernelGGL(token_history_kernel, dim3(cdiv(n, 256), B), dim3(256), 0, (hipStream_t)stream, seen, counts, vocab, (vocab + 31) / 32, ids, ld, n, len);
+    const int words = (vocab + 31) / 32;
+    if (n >= 256 && words * 4 <= 64 * 1024)      // (256 ids against 4752 words of a 152064-token vocabulary: both forms take the same 6 us at 8 rows)
+        hipLaunchKernelGGL(token_history_row_kernel, dim3(B), dim3(1024), words * 4, (hipStream_t)stream, seen, counts, vocab, words, ids, ld, n, len);
+    else hipLaunchKernelGGL(token_history_kernel, dim3(cdiv(n, 256), B), dim3(256), 0, (hipStream_t)stream, seen, counts, vocab, words, ids, ld, n, len);
     SP_CHECK_LAUNCH();
     return SPACER_OK;
 }
@@ -143,11 +192,14 @@ extern "C" int spacer_process_logits(const float* logits, long ld, float* out, l
     SP_REQUIRE(!allowed || (allowed_row ? n_masks > 0 : (n_masks == 1 || n_masks == B)), SPACER_EINVAL, "process_logits: %d masks for %d rows", n_masks, B);
     const bool in_place = logits == out && ld == ld_out;
     LogitArgs A = {logits, out, ld, ld_out, ld_bias, vocab, (vocab + 31) / 32, seen, counts, allowed, allowed_row, n_masks, repetition, frequency, presence,
-                   repetition_dev, frequency_dev, presence_dev, bias, in_place ? 1 : 0};
+                   repetition_dev, frequency_dev, presence_dev, bias};
     const bool vec = (((uintptr_t)logits | (uintptr_t)out | (uintptr_t)bias) & 15) == 0 && ((ld | ld_out | (bias ? ld_bias : 0)) & 3) == 0;
     const dim3 grid(cdiv(vocab, 256 * 4 * LU), B);
-    if (vec) hipLaunchKernelGGL(process_logits_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, A);
-    else hipLaunchKernelGGL(process_logits_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, A);
+    hipStream_t s = (hipStream_t)stream;
+    if (vec && in_place) hipLaunchKernelGGL((process_logits_kernel<true, true>), grid, dim3(256), 0, s, A);
+    else if (vec) hipLaunchKernelGGL((process_logits_kernel<true, false>), grid, dim3(256), 0, s, A);
+    else if (in_place) hipLaunchKernelGGL((process_logits_kernel<false, true>), grid, dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((process_logits_kernel<false, false>), grid, dim3(256), 0, s, A);
     SP_CHECK_LAUNCH();
     return SPACER_OK;
 }

@@ -461,16 +461,22 @@ def _require(ok, what: str) -> None:
         raise SpacerError(what)
 
 
-def _on_current_device(*tensors) -> None:
-    """The launch goes to the current device's current stream: a tensor of another device is refused, not read across the link."""
+def _launch_stream(*tensors) -> int:
+    """The current device's current stream, as a number.  Every tensor has to live on that device: one on another device (or on the host) is
+    refused, not read across the link.  (These entries are called with microseconds of work: no object is made for a stream or a pointer.)"""
     cur = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != cur:
-            raise SpacerError(f"tensor on {t.device}, but the current device is cuda:{cur} (use torch.cuda.device)")
+        if t is not None and t.get_device() != cur:
+            raise SpacerError(f"tensor on {t.device}, but the current device is cuda:{cur} (kernels run on the current device; there is no CPU path)")
+    return torch._C._cuda_getCurrentRawStream(cur)
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _i32(t, n, what: str) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
         raise SpacerError(f"{what}: expected {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
 
 
@@ -487,7 +493,7 @@ class KVCache:
         int8            scale = max|row| / 127, codes -127 .. 127, ties of x / scale to even
     A row that holds a NaN or an infinity gets scale NaN.  The object only describes the tensors (and keeps them alive)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "kv_heads", "capacity", "head_dim", "dtype", "device", "_c", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "kv_heads", "capacity", "head_dim", "dtype", "device", "_c", "_ref", "_shape")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
         _require(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and k.device == v.device,
@@ -517,6 +523,7 @@ class KVCache:
                                stride_seq=stride[0], stride_head=stride[1], stride_pos=stride[2],
                                scale_stride_seq=sstride[0], scale_stride_head=sstride[1], scale_stride_pos=sstride[2])
         self._ref = C.byref(self._c)
+        self._shape = (n, h, cap, d, k.dtype)
 
     @classmethod
     def empty(cls, n_seq: int, capacity: int, kv_heads: int, head_dim: int, dtype="e4m3", device="cuda") -> "KVCache":
@@ -531,71 +538,88 @@ class KVCache:
 
 
 def _kv_source(cache: KVCache, k, v, what: str) -> int:
-    _require(k.dtype == v.dtype == BF16 and k.dim() == v.dim() == 2 and k.shape == v.shape and k.shape[1] == cache.kv_heads * cache.head_dim
-             and k.stride() == v.stride() and (k.stride(1) == 1 or k.shape[0] == 0),
-             f"{what}: k and v must be bf16 [tokens, kv_heads * head_dim] row-major views with the same strides")
-    _on_current_device(cache.k, k, v)
-    return k.stride(0)
+    """Number of rows of the source; k and v are alike."""
+    rows, cols = k.shape if k.dim() == 2 else (0, 0)
+    if (k.dtype != BF16 or v.dtype != BF16 or cols != cache.kv_heads * cache.head_dim or v.shape != k.shape or v.stride() != k.stride()
+            or (rows and k.stride(1) != 1)):
+        raise SpacerError(f"{what}: k and v must be bf16 [tokens, kv_heads * head_dim] row-major views with the same strides")
+    return rows
 
 
 def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor) -> KVCache:
     """Slot (sequence s, position t) of the cache takes row rows[s * capacity + t] (int32) of k / v (bf16 [tokens, kv_heads * head_dim]
     views, e.g. columns of packed q|k|v rows), rounded to the cache's format; a row number below 0 or past the last token leaves the slot
     as it is.  Several slots may name one row."""
-    ld = _kv_source(cache, k, v, "kv_write")
+    n = _kv_source(cache, k, v, "kv_write")
     _i32(rows, cache.n_seq * cache.capacity, "kv_write: rows")
-    _on_current_device(rows)
-    check(_lib.load().spacer_kv_write(cache._ref, _ptr(k), _ptr(v), ld, k.shape[0], _ptr(rows), _stream()), "kv_write")
+    stream = _launch_stream(cache.k, k, v, rows)
+    check(_lib.load().spacer_kv_write(cache._ref, k.data_ptr(), v.data_ptr(), k.stride(0), n, rows.data_ptr(), stream), "kv_write")
     return cache
 
 
 def _kv_lengths(t: torch.Tensor, n: int, what: str) -> int:
     """1 when ``t`` holds one length per sequence, 0 when one for all of them."""
-    _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() in (1, n), f"{what}: expected 1 or {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
-    _on_current_device(t)
-    return int(t.numel() == n and n > 1)
+    m = t.numel()
+    if t.dtype != torch.int32 or not (m == n or m == 1) or not t.is_contiguous():
+        raise SpacerError(f"{what}: expected 1 or {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
+    return int(m == n and n > 1)
 
 
 def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor) -> KVCache:
     """The newest N = tokens / n_seq tokens of every sequence: row s * N + i of k / v (as in ``kv_write``) goes to position lengths[s] + i
     of sequence s (``lengths`` int32 on the device: [n_seq], or [1] for all).  Positions outside the cache are dropped."""
-    ld = _kv_source(cache, k, v, "kv_append")
-    _require(k.shape[0] % cache.n_seq == 0, f"kv_append: {k.shape[0]} rows for {cache.n_seq} sequences")
+    n = _kv_source(cache, k, v, "kv_append")
+    _require(n % cache.n_seq == 0, f"kv_append: {n} rows for {cache.n_seq} sequences")
     per = _kv_lengths(lengths, cache.n_seq, "kv_append: lengths")
-    check(_lib.load().spacer_kv_append(cache._ref, _ptr(k), _ptr(v), ld, k.shape[0] // cache.n_seq, _ptr(lengths), per, _stream()), "kv_append")
+    stream = _launch_stream(cache.k, k, v, lengths)
+    check(_lib.load().spacer_kv_append(cache._ref, k.data_ptr(), v.data_ptr(), k.stride(0), n // cache.n_seq, lengths.data_ptr(), per, stream), "kv_append")
     return cache
 
 
 def kv_read(cache: KVCache, lengths: Optional[torch.Tensor] = None, *, dtype=BF16):
     """(k, v) [n_seq, capacity, kv_heads, head_dim] in bf16 or fp32: the values that the cache stands for.  ``lengths`` (int32 [n_seq]): positions at
     and behind a sequence's length come back as zeros."""
-    _require(dtype in (BF16, torch.float32), f"kv_read: dtype {dtype} (bfloat16 or float32)")
-    _on_current_device(cache.k)
+    f32 = dtype == torch.float32
+    _require(f32 or dtype == BF16, f"kv_read: dtype {dtype} (bfloat16 or float32)")
     if lengths is not None:
         _i32(lengths, cache.n_seq, "kv_read: lengths")
-        _on_current_device(lengths)
+    stream = _launch_stream(cache.k, lengths)
     shape = (cache.n_seq, cache.capacity, cache.kv_heads, cache.head_dim)
-    k, v = torch.empty(shape, device=cache.device, dtype=dtype), torch.empty(shape, device=cache.device, dtype=dtype)
-    check(_lib.load().spacer_kv_read(cache._ref, _ptr(lengths), _ptr(k), _ptr(v), int(dtype == torch.float32), _stream()), "kv_read")
+    k = torch.empty(shape, device=cache.device, dtype=dtype)
+    v = torch.empty_like(k)
+    check(_lib.load().spacer_kv_read(cache._ref, _addr(lengths), k.data_ptr(), v.data_ptr(), int(f32), stream), "kv_read")
     return k, v
 
 
 def decode_qkv_finish_cache(acc32, bias, cos, sin, q_out, cache: KVCache, tail_len, Hq, *, rowss=None, rowss_zero=None, norm_cols=0, eps=0.0):
     """decode_qkv_finish (or with ``rowss``: decode_qkv_finish_normed) with K and V going to position ``tail_len`` of ``cache`` in its format."""
     B, D = cache.n_seq, cache.head_dim
-    _require(acc32.dtype == torch.float32 and acc32.is_contiguous() and tuple(acc32.shape) == (B, (Hq + 2 * cache.kv_heads) * D)
-             and cos.shape == sin.shape == (B, D) and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+    width = (Hq + 2 * cache.kv_heads) * D
+    _require(acc32.dtype == torch.float32 and acc32.is_contiguous() and tuple(acc32.shape) == (B, width)
+             and tuple(cos.shape) == tuple(sin.shape) == (B, D) and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
              and q_out.dtype == BF16 and q_out.is_contiguous() and tuple(q_out.shape) == (B, Hq * D),
              "decode_qkv_finish_cache: acc32 fp32 [B, (Hq + 2 kv_heads) * D], cos / sin fp32 [B, D], q_out bf16 [B, Hq * D], all contiguous")
-    _on_current_device(acc32, bias, cos, sin, q_out, cache.k, rowss, rowss_zero)
+    _require(bias is None or (bias.dtype == BF16 and bias.is_contiguous() and bias.numel() == width), "decode_qkv_finish_cache: bias must be contiguous bf16 [(Hq + 2 kv_heads) * D]")
+    for t in (rowss, rowss_zero):
+        _require(t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= B), "decode_qkv_finish_cache: rowss and rowss_zero must be contiguous fp32 [B]")
     per = _kv_lengths(tail_len, B, "decode_qkv_finish_cache: tail_len")
-    check(_lib.load().spacer_decode_qkv_finish_cache(_ptr(acc32), _ptr(bias), _ptr(cos), _ptr(sin), _ptr(q_out), cache._ref, _ptr(tail_len), per,
-                                                     _ptr(rowss), _ptr(rowss_zero), norm_cols, eps, Hq, _stream()), "decode_qkv_finish_cache")
+    stream = _launch_stream(acc32, bias, cos, sin, q_out, cache.k, tail_len, rowss, rowss_zero)
+    check(_lib.load().spacer_decode_qkv_finish_cache(acc32.data_ptr(), _addr(bias), cos.data_ptr(), sin.data_ptr(), q_out.data_ptr(), cache._ref, tail_len.data_ptr(),
+                                                     per, _addr(rowss), _addr(rowss_zero), norm_cols, eps, Hq, stream), "decode_qkv_finish_cache")
+
+
+_ATTN_CACHE_WS = {}      # workspace sizes by shape: the plan of a launch depends on the shapes alone
 
 
 def attn_cache_workspace_bytes(prompt: Optional[KVCache], tail: Optional[KVCache], rows: int, B: int, nodes: int, Hq: int) -> int:
-    n = int(_lib.load().spacer_attn_cache_workspace_bytes(prompt._ref if prompt is not None else None, tail._ref if tail is not None else None, rows, B, nodes, Hq))
-    check(min(n, 0), "attn_cache_workspace_bytes")
+    key = (prompt._shape if prompt is not None else None, tail._shape if tail is not None else None, rows, B, nodes, Hq)
+    n = _ATTN_CACHE_WS.get(key)
+    if n is None:
+        n = int(_lib.load().spacer_attn_cache_workspace_bytes(prompt._ref if prompt is not None else None, tail._ref if tail is not None else None, rows, B, nodes, Hq))
+        check(min(n, 0), "attn_cache_workspace_bytes")
+        if len(_ATTN_CACHE_WS) > 4096:
+            _ATTN_CACHE_WS.clear()
+        _ATTN_CACHE_WS[key] = n
     return n
 
 
@@ -610,34 +634,40 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
     ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` sequences from
     p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt each.
     prompt_len int32 [n_prompts]; tail_len int32 [B] or [1].  ``workspace``: attn_cache_workspace_bytes bytes; None allocates it."""
-    _require(prompt is not None or tail is not None, "attn_cache: a prompt or a tail cache is needed")
     c = prompt if prompt is not None else tail
-    _require(q.dtype == BF16 and q.dim() == 2 and q.shape[1] == Hq * c.head_dim and q.stride(1) == 1 and nodes >= 1 and q.shape[0] % nodes == 0,
-             f"attn_cache: q must be bf16 [B * nodes, Hq * head_dim] with contiguous rows, got {tuple(q.shape)} {q.dtype}, {nodes} nodes")
-    B = q.shape[0] // nodes
-    _on_current_device(q, c.k, tail.k if tail is not None else None, row0, tree, out, workspace)
-    per = 0
+    if c is None:
+        raise SpacerError("attn_cache: a prompt or a tail cache is needed")
+    rows_q, width = q.shape if q.dim() == 2 else (0, 0)
+    if q.dtype != BF16 or width != Hq * c.head_dim or nodes < 1 or rows_q % nodes or q.stride(1) != 1:
+        raise SpacerError(f"attn_cache: q must be bf16 [B * nodes, Hq * head_dim] with contiguous rows, got {tuple(q.shape)} {q.dtype}, {nodes} nodes")
+    B = rows_q // nodes
+    pr = plen = r0 = tl = tlen = None
+    per = tree_per = 0
     if prompt is not None:
         _i32(prompt_len, prompt.n_seq, "attn_cache: prompt_len")
-        _on_current_device(prompt_len)
+        pr, plen = prompt._ref, prompt_len.data_ptr()
         if row0 is not None:
             _i32(row0, prompt.n_seq + 1, "attn_cache: row0")
+            r0 = row0.data_ptr()
     if tail is not None:
         per = _kv_lengths(tail_len, B, "attn_cache: tail_len")
-    tree_per = 0
+        tl, tlen = tail._ref, tail_len.data_ptr()
     if tree is not None:
-        _require(tree.dtype == torch.int64 and tree.is_contiguous() and tuple(tree.shape) in ((nodes,), (B, nodes)),
-                 f"attn_cache: tree must be contiguous int64 [{nodes}] or [{B}, {nodes}], got {tuple(tree.shape)} {tree.dtype}")
-        tree_per = int(tree.dim() == 2)
+        tree_per = tree.dim() - 1
+        if tree.dtype != torch.int64 or not tree.is_contiguous() or tuple(tree.shape) not in ((nodes,), (B, nodes)):
+            raise SpacerError(f"attn_cache: tree must be contiguous int64 [{nodes}] or [{B}, {nodes}], got {tuple(tree.shape)} {tree.dtype}")
+    stream = _launch_stream(q, prompt and prompt.k, prompt and prompt_len, row0, tail and tail.k, tail and tail_len, tree, out, workspace)
     if out is None:
-        out = torch.empty(q.shape[0], Hq * c.head_dim, device=q.device, dtype=BF16)
-    _require(out.dtype == BF16 and out.is_contiguous() and tuple(out.shape) == (q.shape[0], Hq * c.head_dim), "attn_cache: out must be contiguous bf16 [B * nodes, Hq * head_dim]")
+        out = torch.empty((rows_q, width), device=q.device, dtype=BF16)
+    elif out.dtype != BF16 or tuple(out.shape) != (rows_q, width) or not out.is_contiguous():
+        raise SpacerError("attn_cache: out must be contiguous bf16 [B * nodes, Hq * head_dim]")
     if workspace is None:
-        workspace = torch.empty(attn_cache_workspace_bytes(prompt, tail, rows_per_prompt, B, nodes, Hq), device=q.device, dtype=torch.uint8)
-    check(_lib.load().spacer_attn_cache(_ptr(q), q.stride(0), prompt._ref if prompt is not None else None, _ptr(prompt_len) if prompt is not None else None,
-                                        _ptr(row0) if prompt is not None else None, rows_per_prompt, tail._ref if tail is not None else None,
-                                        _ptr(tail_len) if tail is not None else None, per, _ptr(tree), tree_per, _ptr(out), B, nodes, Hq, scale,
-                                        _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()), "attn_cache")
+        n = attn_cache_workspace_bytes(prompt, tail, rows_per_prompt, B, nodes, Hq)
+        workspace = torch.empty(n, device=q.device, dtype=torch.uint8)
+    else:
+        n = workspace.numel() * workspace.element_size()
+    check(_lib.load().spacer_attn_cache(q.data_ptr(), q.stride(0), pr, plen, r0, rows_per_prompt, tl, tlen, per, _addr(tree), tree_per, out.data_ptr(), B, nodes, Hq,
+                                        scale, workspace.data_ptr(), n, stream), "attn_cache")
     return out
 
 
@@ -648,35 +678,37 @@ def token_history(B: int, vocab: int, device):
 
 
 def _history(seen, counts, B, vocab, what):
-    _require(seen.dtype == torch.int32 and seen.is_contiguous() and tuple(seen.shape) == (B, (vocab + 31) // 32),
-             f"{what}: seen must be contiguous int32 [{B}, {(vocab + 31) // 32}], got {tuple(seen.shape)} {seen.dtype}")
-    _require(counts is None or (counts.dtype == torch.int32 and counts.is_contiguous() and tuple(counts.shape) == (B, vocab)),
-             f"{what}: counts must be contiguous int32 [{B}, {vocab}]")
+    words = (vocab + 31) // 32
+    if seen.dtype != torch.int32 or tuple(seen.shape) != (B, words) or not seen.is_contiguous():
+        raise SpacerError(f"{what}: seen must be contiguous int32 [{B}, {words}], got {tuple(seen.shape)} {seen.dtype}")
+    if counts is not None and (counts.dtype != torch.int32 or tuple(counts.shape) != (B, vocab) or not counts.is_contiguous()):
+        raise SpacerError(f"{what}: counts must be contiguous int32 [{B}, {vocab}], got {tuple(counts.shape)} {counts.dtype}")
 
 
 def token_history_add_(seen, counts, ids, lengths=None, *, vocab: Optional[int] = None):
     """Marks ids[b, i] (int64 [B, n], i < lengths[b] where given) as seen in row b and counts them; ``counts`` None only marks (prompt tokens:
     the repetition penalty asks what has been seen, the frequency and presence penalties what has been generated).  Ids outside the vocabulary
     are skipped.  ``vocab``: needed without ``counts`` when it is not a multiple of 32."""
-    _require(ids.dtype == torch.int64 and ids.dim() == 2 and (ids.stride(1) == 1 or ids.shape[1] <= 1), f"token_history_add_: ids must be int64 [B, n] with contiguous rows, got {tuple(ids.shape)} {ids.dtype}")
+    if ids.dtype != torch.int64 or ids.dim() != 2 or (ids.shape[1] > 1 and ids.stride(1) != 1):
+        raise SpacerError(f"token_history_add_: ids must be int64 [B, n] with contiguous rows, got {tuple(ids.shape)} {ids.dtype}")
     B, n = ids.shape
     vocab = vocab if vocab is not None else counts.shape[1] if counts is not None else seen.shape[1] * 32
     _history(seen, counts, B, vocab, "token_history_add_")
     if lengths is not None:
         _i32(lengths, B, "token_history_add_: lengths")
-    _on_current_device(seen, counts, ids, lengths)
-    check(_lib.load().spacer_token_history_add(_ptr(seen), _ptr(counts), B, vocab, _ptr(ids), ids.stride(0), n, _ptr(lengths), _stream()), "token_history_add")
+    stream = _launch_stream(seen, counts, ids, lengths)
+    check(_lib.load().spacer_token_history_add(seen.data_ptr(), _addr(counts), B, vocab, ids.data_ptr(), ids.stride(0), n, _addr(lengths), stream), "token_history_add")
 
 
 def _per_row(x, neutral, B, what):
-    """(number, device pointer) of a penalty given as a number, an fp32 [B] tensor or None."""
+    """(number, device tensor) of a penalty given as a number, an fp32 [B] tensor or None."""
     if x is None:
-        return neutral, _ptr(None)
+        return neutral, None
     if isinstance(x, torch.Tensor):
-        _require(x.dtype == torch.float32 and x.is_contiguous() and tuple(x.shape) == (B,), f"process_logits: {what} must be a number or contiguous fp32 [{B}]")
-        _on_current_device(x)
-        return neutral, _ptr(x)
-    return float(x), _ptr(None)
+        if x.dtype != torch.float32 or tuple(x.shape) != (B,) or not x.is_contiguous():
+            raise SpacerError(f"process_logits: {what} must be a number or contiguous fp32 [{B}]")
+        return neutral, x
+    return float(x), None
 
 
 def process_logits(logits32, *, seen=None, counts=None, repetition=None, frequency=None, presence=None, bias=None, allowed=None, allowed_row=None,
@@ -689,33 +721,37 @@ def process_logits(logits32, *, seen=None, counts=None, repetition=None, frequen
     repetition / frequency / presence: numbers or fp32 [B].  allowed: int32 [n_masks, ceil(vocab / 32)] (bit v % 32 of word v // 32); row b
     takes mask allowed_row[b] (int32 [B], a number outside the table: no mask), or without ``allowed_row`` mask b, or the only one.  A row whose
     mask allows nothing is all -inf: the sampler has nothing to draw there."""
-    _require(logits32.dtype == torch.float32 and logits32.dim() == 2 and logits32.stride(1) == 1, "process_logits: logits must be fp32 [B, vocab] with contiguous rows")
+    if logits32.dtype != torch.float32 or logits32.dim() != 2 or logits32.stride(1) != 1:
+        raise SpacerError("process_logits: logits must be fp32 [B, vocab] with contiguous rows")
     B, vocab = logits32.shape
     if out is None:
         out = logits32
-    _require(out.dtype == torch.float32 and out.shape == logits32.shape and out.stride(1) == 1, "process_logits: out must be fp32 [B, vocab] with contiguous rows")
+    elif out.dtype != torch.float32 or out.shape != logits32.shape or out.stride(1) != 1:
+        raise SpacerError("process_logits: out must be fp32 [B, vocab] with contiguous rows")
     if seen is not None:
         _history(seen, counts, B, vocab, "process_logits")
-    _require(seen is not None or (counts is None and repetition is None), "process_logits: penalties need the history (seen)")
-    words, ld_bias, n_masks = (vocab + 31) // 32, 0, 0
+    elif counts is not None or repetition is not None:
+        raise SpacerError("process_logits: penalties need the history (seen)")
+    ld_bias = n_masks = 0
     if bias is not None:
-        _require(bias.dtype == torch.float32 and tuple(bias.shape) in ((vocab,), (B, vocab)) and bias.stride(-1) == 1,
-                 f"process_logits: bias must be fp32 [{vocab}] or [{B}, {vocab}] with contiguous rows, got {tuple(bias.shape)} {bias.dtype}")
+        if bias.dtype != torch.float32 or tuple(bias.shape) not in ((vocab,), (B, vocab)) or bias.stride(-1) != 1:
+            raise SpacerError(f"process_logits: bias must be fp32 [{vocab}] or [{B}, {vocab}] with contiguous rows, got {tuple(bias.shape)} {bias.dtype}")
         ld_bias = bias.stride(0) if bias.dim() == 2 else 0
     if allowed is not None:
-        _require(allowed.dtype == torch.int32 and allowed.dim() == 2 and allowed.is_contiguous() and allowed.shape[1] == words,
-                 f"process_logits: allowed must be contiguous int32 [n_masks, {words}], got {tuple(allowed.shape)} {allowed.dtype}")
+        words = (vocab + 31) // 32
+        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] != words or not allowed.is_contiguous():
+            raise SpacerError(f"process_logits: allowed must be contiguous int32 [n_masks, {words}], got {tuple(allowed.shape)} {allowed.dtype}")
         n_masks = allowed.shape[0]
         if allowed_row is not None:
             _i32(allowed_row, B, "process_logits: allowed_row")
-    else:
-        _require(allowed_row is None, "process_logits: allowed_row without allowed")
-    _on_current_device(logits32, out, seen, counts, bias, allowed, allowed_row)
-    r, rp = _per_row(repetition, 1.0, B, "repetition")
-    f, fp = _per_row(frequency, 0.0, B, "frequency")
-    p, pp = _per_row(presence, 0.0, B, "presence")
-    check(_lib.load().spacer_process_logits(_ptr(logits32), logits32.stride(0), _ptr(out), out.stride(0), B, vocab, _ptr(seen), _ptr(counts), r, rp, f, fp, p, pp,
-                                            _ptr(bias), ld_bias, _ptr(allowed), n_masks, _ptr(allowed_row), _stream()), "process_logits")
+    elif allowed_row is not None:
+        raise SpacerError("process_logits: allowed_row without allowed")
+    r, rt = _per_row(repetition, 1.0, B, "repetition")
+    f, ft = _per_row(frequency, 0.0, B, "frequency")
+    p, pt = _per_row(presence, 0.0, B, "presence")
+    stream = _launch_stream(logits32, out, seen, counts, bias, allowed, allowed_row, rt, ft, pt)
+    check(_lib.load().spacer_process_logits(logits32.data_ptr(), logits32.stride(0), out.data_ptr(), out.stride(0), B, vocab, _addr(seen), _addr(counts), r, _addr(rt), f,
+                                            _addr(ft), p, _addr(pt), _addr(bias), ld_bias, _addr(allowed), n_masks, _addr(allowed_row), stream), "process_logits")
     return out
 
 

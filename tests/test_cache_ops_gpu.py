@@ -235,6 +235,11 @@ SHAPES = [
     (2, 1, [129, 3], 200, [0, 136], 64, 8, 8, 64),
     (1, 2, [40], 100, [31, 98], 5, 2, 1, 64),          # the second sequence's nodes leave the cache at its end
     (1, 3, [2500], 20, [4, 5, 6], 2, 6, 2, 128),
+    # contexts past the one-launch form, by the columns that share the prompt's and the sequence's keys: 16, 32, 64 and more
+    (1, 2, [700], 33, [5, 32], 1, 6, 2, 128), (1, 2, [800], 33, [5, 32], 1, 6, 2, 64),
+    (1, 1, [600], 40, [3], 7, 12, 3, 128), (1, 1, [900], 40, [33], 7, 12, 3, 64),
+    (2, 1, [600, 555], 100, [0, 36], 64, 16, 2, 128), (2, 1, [33, 640], 100, [31, 36], 33, 6, 2, 64),
+    (2, 4, [520, 1], 1100, [1099, 1000, 64, 63, 0, 500, 999, 31], 1, 28, 4, 64),
 ]
 
 

@@ -42,7 +42,7 @@ def cache(**kw):
 
 
 BAD_CACHES = [dict(struct_bytes=8), dict(format=3), dict(format=-1), dict(head_dim=80), dict(head_dim=0), dict(n_seq=0), dict(capacity=-1), dict(kv_heads=0),
-              dict(k=None), dict(v=0x2008), dict(stride_pos=136), dict(stride_head=8), dict(k_scale=None), dict(v_scale=None),
+              dict(stride_pos=1 << 27), dict(scale_stride_pos=-1), dict(k=None), dict(v=0x2008), dict(stride_pos=136), dict(stride_head=8), dict(k_scale=None), dict(v_scale=None),
               dict(format=_lib.SPACER_KV_BF16, stride_pos=132)]
 
 
@@ -78,9 +78,13 @@ def test_entries_refuse(lib):
                dict(Hq=3), dict(Hq=0), dict(rows=0), dict(rows=2), dict(prompt=C.byref(cache(head_dim=64))), dict(prompt=C.byref(cache(format=1))),
                dict(prompt=C.byref(cache(kv_heads=1)))):
         assert attn(**kw) == EINVAL, kw
-    assert attn(ws=None) == ENOMEM and attn(n=64) == ENOMEM and attn(ws=p + 4) == ENOMEM
+    # (short contexts need no workspace)
+    assert lib.spacer_attn_cache_workspace_bytes(r, r, 1, 2, 1, 4) == 0
+    r = C.byref(cache(capacity=4096, stride_head=4096 * 128, stride_seq=2 * 4096 * 128, scale_stride_head=4096, scale_stride_seq=8192))
     need = lib.spacer_attn_cache_workspace_bytes(r, r, 1, 2, 1, 4)
-    assert need > 0 and attn(n=need - 1) == ENOMEM
+    assert need > 0
+    for kw in (dict(ws=None), dict(n=64), dict(ws=p + 4), dict(n=need - 1)):
+        assert attn(prompt=r, tail=r, **kw) == ENOMEM, kw
 
     def logits(x=p, out=p, B=2, V=100, seen=p, counts=p, rep=1.0, f=0.0, pr=0.0, allowed=None, n=0, row=None):
         return lib.spacer_process_logits(x, 100, out, 100, B, V, seen, counts, rep, None, f, None, pr, None, None, 0, allowed, n, row, None)
