@@ -20,7 +20,6 @@
 namespace {
 
 constexpr int TK = 32;            // keys per wave and step
-constexpr int SOLO_MAX = 512;      // positions
 constexpr float LOG2E = 1.4426950408889634f;
 
 // n / d for 0 <= n < 2^31 by a multiplication (d is the same for a whole launch): m = floor(2^(31 + s) / d) + 1 with 2^s >= d is exact there
@@ -88,11 +87,10 @@ struct Tile {
     static __device__ __forceinline__ int swz(int row) { return (row / (RB >= 256 ? 1 : 256 / RB)) & (CPR - 1); }
 };
 
-// column blocks that the waves join at once: two workgroups' buffers fit a CU's 160 KB
-constexpr int join_blocks(int D, int nc) { return nc < (D == 64 ? 4 : 2) ? nc : (D == 64 ? 4 : 2); }
+// Column blocks of a workgroup: 1 or 2.  (4 leave one lane 128 registers of O: e4m3 rollouts 8 x 8 over 1391 + 300 positions 18.0 instead of 13.8 us, bf16
+// 33 instead of 21; at D = 64 the two are level.)
 constexpr int lds_bytes(int es, int D, int nc) {
-    const int work = 4 * (TK * D * es + 2 * TK * 4) + (nc > 2 ? nc * (D / 32) * 64 * 16 : 0);
-    const int join = join_blocks(D, nc) * 16 * (4 * (D + 4) * 4 + 4 * 8);
+    const int work = 4 * (TK * D * es + 2 * TK * 4), join = nc * 16 * (4 * (D + 4) * 4 + 4 * 8);      // at most 69 KB: two workgroups per CU
     return work > join ? work : join;
 }
 
@@ -108,14 +106,14 @@ struct KeySegment {
 template <int FMT, int D, int NC, class ColInfo>
 struct Columns {
     using T = Tile<FMT, D, NC>;
-    static constexpr int DF = D / 16, QR = NC <= 2 ? NC : 1;
+    static constexpr int DF = D / 16;
 
     const AttnCacheArgs& A;
     const ColInfo& info;
     const int c0, lane, wave, l15, g;
-    char *vimg, *qlds;
+    char* vimg;
     float* sc;
-    bf16x8 qreg[QR][T::STEPS];
+    bf16x8 qreg[NC][T::STEPS];
     f32x4 oacc[NC][DF];
     float m_run[NC], l_run[NC];
     uint4 kr[2][T::KL], vr[T::VL];
@@ -126,7 +124,6 @@ struct Columns {
           g((threadIdx.x & 63) >> 4), scr(0.f) {
         vimg = smem + wave * T::IMG;
         sc = (float*)(smem + 4 * T::IMG) + wave * 2 * TK;
-        qlds = smem + 4 * (T::IMG + 2 * TK * 4);
 #pragma unroll
         for (int cb = 0; cb < NC; ++cb) {
             m_run[cb] = -INFINITY; l_run[cb] = 0.f;
@@ -146,15 +143,10 @@ struct Columns {
         return __builtin_bit_cast(bf16x8, x);
     }
     __device__ __forceinline__ void load_queries() {
-        if (NC <= 2) {
 #pragma unroll
-            for (int cb = 0; cb < QR; ++cb)
+        for (int cb = 0; cb < NC; ++cb)
 #pragma unroll
-                for (int s = 0; s < T::STEPS; ++s) qreg[cb][s] = q_frag(cb, s);
-        } else {
-            for (int f = wave; f < NC * T::STEPS; f += 4) *(bf16x8*)(qlds + (f * 64 + lane) * 16) = q_frag(f / T::STEPS, f % T::STEPS);
-            __syncthreads();
-        }
+            for (int s = 0; s < T::STEPS; ++s) qreg[cb][s] = q_frag(cb, s);
     }
 
     // requests tile t: 64-bit arithmetic stays in scalars, a lane adds 32 bits (32 rows span less than 2^31 bytes: checked on the host).
@@ -221,9 +213,8 @@ struct Columns {
             }
 #pragma unroll
             for (int cb = 0; cb < NC; ++cb) {
-                const bf16x8 qf = NC <= 2 ? qreg[NC <= 2 ? cb : 0][step] : *(const bf16x8*)(qlds + ((cb * T::STEPS + step) * 64 + lane) * 16);
-                st[cb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[0], qf, st[cb][0], 0, 0, 0);
-                st[cb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[1], qf, st[cb][1], 0, 0, 0);
+                st[cb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[0], qreg[cb][step], st[cb][0], 0, 0, 0);
+                st[cb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[1], qreg[cb][step], st[cb][1], 0, 0, 0);
             }
         }
         if (t + 4 < s.t1) fetch(s, t + 4);                // the registers of K and V are free: the next tile is under way during the rest
@@ -337,53 +328,49 @@ struct Columns {
         }
     }
 
-    // joins the waves, RC blocks of 16 columns at a time ([wave][column][D + 4 floats], [wave][column] (m, l) in LDS), and writes the record `slot` of
-    // every column, or with slot < 0 its output
+    // joins the waves ([wave][column][D + 4 floats], [wave][column] (m, l) in LDS) and writes the record `slot` of every column, or with slot < 0 its output
     __device__ __forceinline__ void finish(char* smem, int slot) {
-        constexpr int RC = join_blocks(D, NC), JC = RC * 16, TPC = 256 / JC, PER = D / TPC;      // columns, threads per column, floats per thread
+        constexpr int JC = NC * 16, TPC = 256 / JC, PER = D / TPC;      // columns, threads per column, floats per thread
         const int tid = threadIdx.x;
         float* jo = (float*)smem;
         float2* jm = (float2*)(smem + 4 * JC * (D + 4) * 4);
         const int jc = tid / TPC, jd = (tid % TPC) * 4;       // (a thread's float4 lie TPC * 4 floats apart: neighbouring threads, neighbouring banks)
         const long ncol_all = (long)A.B * A.N * A.Hq;
+        __syncthreads();
 #pragma unroll
-        for (int cb = 0; cb < NC; cb += RC) {
-            __syncthreads();
+        for (int r = 0; r < NC; ++r) {
+            float l = l_run[r];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
 #pragma unroll
-            for (int r = 0; r < RC; ++r) {
-                float l = l_run[cb + r];
-                l += __shfl_xor(l, 16, 64);
-                l += __shfl_xor(l, 32, 64);
-#pragma unroll
-                for (int df = 0; df < DF; ++df)
-                    *(f32x4*)(jo + (wave * JC + r * 16 + l15) * (D + 4) + df * 16 + g * 4) = oacc[cb + r][df];
-                if (g == 0) jm[wave * JC + r * 16 + l15] = make_float2(m_run[cb + r], l);
-            }
-            __syncthreads();
-            int row, head, node;
-            if (!info(c0 + cb * 16 + jc, row, head, node)) continue;
-            float M = -INFINITY, L = 0.f, f[4];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * JC + jc].x);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float2 ml = jm[w * JC + jc];
-                f[w] = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
-                L += ml.y * f[w];
-            }
-            const long col = ((long)row * A.N + node) * A.Hq + head;
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-            for (int i = 0; i < PER / 4; ++i) {
-                const int d = jd + i * TPC * 4;
-                f32x4 O = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) O += *(const f32x4*)(jo + (w * JC + jc) * (D + 4) + d) * f[w];
-                if (slot < 0) *(uint2*)(A.o + col * D + d) = make_uint2(pack_bf2(O[0] * inv, O[1] * inv), pack_bf2(O[2] * inv, O[3] * inv));
-                else *(f32x4*)(A.rec_o + ((long)slot * ncol_all + col) * D + d) = O;
-            }
-            if (slot >= 0 && tid % TPC == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
+            for (int df = 0; df < DF; ++df)
+                *(f32x4*)(jo + (wave * JC + r * 16 + l15) * (D + 4) + df * 16 + g * 4) = oacc[r][df];
+            if (g == 0) jm[wave * JC + r * 16 + l15] = make_float2(m_run[r], l);
         }
+        __syncthreads();
+        int row, head, node;
+        if (!info(c0 + jc, row, head, node)) return;
+        float M = -INFINITY, L = 0.f, f[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * JC + jc].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 ml = jm[w * JC + jc];
+            f[w] = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+            L += ml.y * f[w];
+        }
+        const long col = ((long)row * A.N + node) * A.Hq + head;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int i = 0; i < PER / 4; ++i) {
+            const int d = jd + i * TPC * 4;
+            f32x4 O = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) O += *(const f32x4*)(jo + (w * JC + jc) * (D + 4) + d) * f[w];
+            if (slot < 0) *(uint2*)(A.o + col * D + d) = make_uint2(pack_bf2(O[0] * inv, O[1] * inv), pack_bf2(O[2] * inv, O[3] * inv));
+            else *(f32x4*)(A.rec_o + ((long)slot * ncol_all + col) * D + d) = O;
+        }
+        if (slot >= 0 && tid % TPC == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
     }
     // no keys: the columns' records say so by their maximum alone
     __device__ __forceinline__ void finish_empty(int slot) const {
@@ -556,46 +543,43 @@ struct AttnPlan {
     long cols;
 };
 
-// Column blocks: as wide as the columns need, up to 64 (a wave's fp32 O of 64 x 128 is 128 registers).
-// Key ranges: the pair (sa, sb) whose estimated time is least: 512 workgroups run at once (two per CU); one costs its 32-key tiles per wave, a wide
-// tile about twice a narrow one, and some 4 tiles for its start and its end.  The capacities stand for the lengths, which only the device knows; half of
-// the tail's, which fills up while a rollout runs.
-// Solo: contexts of up to 512 positions (16 tiles, 4 per wave) in one launch without records.
+// How a launch is cut, from the shapes alone (the capacities stand for the lengths, which only the device knows; half of the tail's, which fills up while a
+// rollout runs).
+// Short contexts go in one launch: 640 positions, or 1024 where that launch has 128 workgroups or more (one launch | two: 6.3 | 7.6 us at 384
+// positions of 1 x 2 rollouts, 9.5 | 8.7 at 1024; 8 x 8 rollouts 11.1 | 13.4 us at 1024, 15.3 | 14.5 at 1536).
+// Others: of the widths (16 or 32 columns) and numbers of key ranges (sa, sb) the one whose estimate is least.  The estimate's constants (us) were fitted
+// to 1100 launches of 45 shapes (1 to 8 prompts, 1 to 2048 columns, 300 to 14000 positions, all formats): the choice is 4 % behind the best of them in the
+// mean, 8 % with a fixed width of 32.  Two workgroups per CU run at once; a third round rarely ends together with the second.
 AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
     const spacer_kv_cache* c = prompt ? prompt : tail;
-    const int rep = Hq / c->kv_heads;
-    const long ca = prompt ? (long)rows * N * rep : 0, cb = (long)N * rep;
-    AttnPlan p;
+    const long rep = Hq / c->kv_heads, cb = N * rep, ca = prompt ? rows * cb : 0, most = ca > cb ? ca : cb;
+    const long positions = (long)(prompt ? prompt->capacity : 0) + (tail ? tail->capacity : 0), narrow = (long)B * c->kv_heads * cdiv(cb, 16);
+    AttnPlan p = {};
     p.cols = (long)B * N * Hq;
-    p.solo = (long)(prompt ? prompt->capacity : 0) + (tail ? tail->capacity : 0) <= SOLO_MAX;
+    p.solo = positions <= (narrow >= 128 ? 1024 : 640);
     if (p.solo) {
-        p.nca = p.ncb = cb <= 16 ? 1 : cb <= 32 ? 2 : 4;
-        p.cba = 0; p.cbb = cdiv(cb, 16 * p.ncb);
-        p.sa = p.sb = 0;
+        p.ncb = cb <= 16 || narrow <= 512 ? 1 : 2;
+        p.cbb = cdiv(cb, 16 * p.ncb);
         return p;
     }
-    const long cbt = tail ? cb : 0, most = ca > cbt ? ca : cbt;
-    if (most <= 16) p.nca = p.ncb = 1;
-    else if (cbt <= 16) { p.nca = 4; p.ncb = 1; }
-    else if (most <= 32) p.nca = p.ncb = 2;
-    else p.nca = p.ncb = 4;
-    p.cba = prompt ? cdiv(ca, 16 * p.nca) : 0;
-    p.cbb = tail ? cdiv(cbt, 16 * p.ncb) : 0;
-    const double ja = prompt ? (double)prompt->n_seq * c->kv_heads * p.cba : 0, jb = tail ? (double)B * c->kv_heads * p.cbb : 0;
-    const double ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
-    const double wa = 0.5 + 0.5 * p.nca, wb = 0.5 + 0.5 * p.ncb, start = 4.0;
+    static const int ranges[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
+    const double start = 36.0, once = 3.8, ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
     double best = 1e300;
-    p.sa = prompt ? 1 : 0; p.sb = tail ? 1 : 0;
-    for (int sb = tail ? 1 : 0; sb <= (tail ? 4 : 0); ++sb) {
-        if (sb > 1 && tb / sb < 2) break;
-        for (int sa = prompt ? 1 : 0; sa <= (prompt ? 64 : 0); sa += sa < 16 ? 1 : 4) {
-            if (sa > 1 && ta / sa < 1) break;
-            const double a = sa ? start + ceil(ta / sa) * wa : 0, b = sb ? start + ceil(tb / sb) * wb : 0, longest = a > b ? a : b;
-            const double blocks = ja * sa + jb * sb, work = (ja * sa * a + jb * sb * b) / 512;
-            double t = work > longest ? work : longest;
-            if (blocks > 512) t += 0.25 * (a > b && b > 0 ? b : a > 0 ? a : b);          // a second round rarely ends together
-            t += 0.15 * (sa + sb);                                                       // records to write and join
-            if (t < best - 1e-9) { best = t; p.sa = sa; p.sb = sb; }
+    for (int nc = 1; nc <= (most > 16 ? 2 : 1); ++nc) {
+        const int ncb = cb <= 16 ? 1 : nc, cba = prompt ? cdiv(ca, 16 * nc) : 0, cbb = tail ? cdiv(cb, 16 * ncb) : 0;
+        const double ja = (prompt ? (double)prompt->n_seq : 0) * c->kv_heads * cba, jb = (double)B * c->kv_heads * cbb;
+        for (int ia = 0; ia < 13; ++ia) {
+            const int sa = prompt ? ranges[ia] : 0;
+            if (ia > 0 && (!prompt || ta < sa)) break;
+            for (int sb = tail ? 1 : 0; sb <= (tail ? 4 : 0); sb = sb ? 2 * sb : 1) {
+                if (sb > 1 && tb < sb) break;
+                const double a = sa ? ceil(ta / sa) * (0.21 + 0.155 * nc) : 0, b = sb ? ceil(tb / sb) * (0.21 + 0.155 * ncb) : 0;
+                const double work = 0.5 * start + (ja * sa * (once + a) + jb * sb * (once + b)) / 512, longest = start + (a > b ? a : b);
+                double t = work > longest ? work : longest;
+                if (ja * sa + jb * sb > 512) t += 0.95 * (start + (sa && sb ? (a < b ? a : b) : a + b));
+                t += 2e-4 * p.cols * (sa + sb) + 1.15 * cdiv(sa + sb, 8);
+                if (t < best) { best = t; p.nca = nc; p.ncb = ncb; p.cba = cba; p.cbb = cbb; p.sa = sa; p.sb = sb; }
+            }
         }
     }
     return p;
@@ -677,8 +661,7 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
 #define CALL(F, DD)                                                                                                                                 \
     do {                                                                                                                                            \
         if (p.ncb == 1) LAUNCH(F, DD, 1);                                                                                                           \
-        else if (p.ncb == 2) LAUNCH(F, DD, 2);                                                                                                      \
-        else LAUNCH(F, DD, 4);                                                                                                                      \
+        else LAUNCH(F, DD, 2);                                                                                                                      \
     } while (0)
         KV_DISPATCH(c, CALL);
 #undef CALL
@@ -700,9 +683,8 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
 #define CALL(F, DD)                                                                                                                                 \
     do {                                                                                                                                            \
         if (p.nca == 1) LAUNCH(F, DD, 1, 1);                                                                                                        \
-        else if (p.nca == 2) LAUNCH(F, DD, 2, 2);                                                                                                   \
-        else if (p.ncb == 1) LAUNCH(F, DD, 4, 1);                                                                                                   \
-        else LAUNCH(F, DD, 4, 4);                                                                                                                   \
+        else if (p.ncb == 1) LAUNCH(F, DD, 2, 1);                                                                                                   \
+        else LAUNCH(F, DD, 2, 2);                                                                                                                   \
     } while (0)
     KV_DISPATCH(c, CALL);
 #undef CALL

@@ -658,16 +658,17 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
             raise SpacerError(f"attn_cache: tree must be contiguous int64 [{nodes}] or [{B}, {nodes}], got {tuple(tree.shape)} {tree.dtype}")
     stream = _launch_stream(q, prompt and prompt.k, prompt and prompt_len, row0, tail and tail.k, tail and tail_len, tree, out, workspace)
     if out is None:
-        out = torch.empty((rows_q, width), device=q.device, dtype=BF16)
+        out = q.new_empty((rows_q, width))
     elif out.dtype != BF16 or tuple(out.shape) != (rows_q, width) or not out.is_contiguous():
         raise SpacerError("attn_cache: out must be contiguous bf16 [B * nodes, Hq * head_dim]")
     if workspace is None:
         n = attn_cache_workspace_bytes(prompt, tail, rows_per_prompt, B, nodes, Hq)
-        workspace = torch.empty(n, device=q.device, dtype=torch.uint8)
+        if n:
+            workspace = torch.empty(n, device=q.device, dtype=torch.uint8)
     else:
         n = workspace.numel() * workspace.element_size()
     check(_lib.load().spacer_attn_cache(q.data_ptr(), q.stride(0), pr, plen, r0, rows_per_prompt, tl, tlen, per, _addr(tree), tree_per, out.data_ptr(), B, nodes, Hq,
-                                        scale, workspace.data_ptr(), n, stream), "attn_cache")
+                                        scale, _addr(workspace), n, stream), "attn_cache")
     return out
 
 
