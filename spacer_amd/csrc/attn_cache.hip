@@ -45,14 +45,15 @@ struct AttnCacheArgs {
     bf16_t* o;
 };
 
+// eight codes as bf16, exact; e4m3 codes times their row's scale, a power of two
 template <int FMT>
-__device__ __forceinline__ bf16x8 codes_to_bf16(uint2 w) {
+__device__ __forceinline__ bf16x8 codes_to_bf16(uint2 w, float s) {
     uint32_t o[4];
     if (FMT == KV_E4M3) {
-        o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, false));
-        o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, true));
-        o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, false));
-        o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, true));
+        o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, false));
+        o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, true));
+        o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, false));
+        o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, true));
     } else {
         const uint32_t a[2] = {w.x, w.y};
 #pragma unroll
@@ -117,11 +118,11 @@ struct Columns {
     f32x4 oacc[NC][DF];
     float m_run[NC], l_run[NC];
     uint4 kr[2][T::KL], vr[T::VL];
-    float scr;
+    float scr, kscr[2];               // row scales: of V (lanes 32 .., e4m3: all lanes) and of K (int8: lanes .. 31; e4m3: kscr, a lane's own rows)
 
     __device__ __forceinline__ Columns(const AttnCacheArgs& args, const ColInfo& ci, char* smem, int first)
         : A(args), info(ci), c0(first), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
-          g((threadIdx.x & 63) >> 4), scr(0.f) {
+          g((threadIdx.x & 63) >> 4), scr(0.f), kscr{1.f, 1.f} {
         vimg = smem + wave * T::IMG;
         sc = (float*)(smem + 4 * T::IMG) + wave * 2 * TK;
 #pragma unroll
@@ -149,28 +150,34 @@ struct Columns {
             for (int s = 0; s < T::STEPS; ++s) qreg[cb][s] = q_frag(cb, s);
     }
 
-    // requests tile t: 64-bit arithmetic stays in scalars, a lane adds 32 bits (32 rows span less than 2^31 bytes: checked on the host).
+    // Requests for tile t: 64-bit arithmetic stays in scalars, a lane adds 32 bits (32 rows span less than 2^31 bytes: checked on the host).
     // Keys behind the last repeat it, so every address lies inside the cache.
-    __device__ __forceinline__ void fetch(const KeySegment& s, int t) {
+    __device__ __forceinline__ void fetch_k(const KeySegment& s, int t) {
         const int k0 = t * TK, last = s.total - 1 - k0;
-        const char *kb = s.k + (long)k0 * s.row_b, *vb = s.v + (long)k0 * s.row_b;
-        const bool full = last >= TK - 1;
+        const char* kb = s.k + (long)k0 * s.row_b;
 #pragma unroll
         for (int kf = 0; kf < 2; ++kf) {
-            const uint32_t off = (uint32_t)((full ? kf * 16 + l15 : min(kf * 16 + l15, last)) * s.row_b + g * 16);
+            const int row = last >= TK - 1 ? kf * 16 + l15 : min(kf * 16 + l15, last);
+            const uint32_t off = (uint32_t)(row * s.row_b + g * 16);
 #pragma unroll
             for (int h = 0; h < T::KL; ++h) kr[kf][h] = *(const uint4*)(kb + off + h * 64);
+            if (FMT == KV_E4M3) kscr[kf] = s.ks[(long)k0 * s.c_pos + row * s.c_pos];
         }
+    }
+    __device__ __forceinline__ void fetch_v(const KeySegment& s, int t) {
+        const int k0 = t * TK, last = s.total - 1 - k0;
+        const char* vb = s.v + (long)k0 * s.row_b;
         if (FMT != KV_BF16) {
-            const float* sb = (lane < TK ? s.ks : s.vs) + (long)k0 * s.c_pos;
+            const float* sb = (FMT == KV_E4M3 || lane >= TK ? s.vs : s.ks) + (long)k0 * s.c_pos;
             scr = sb[min(lane & (TK - 1), last) * s.c_pos];
         }
 #pragma unroll
         for (int i = 0; i < T::VL; ++i) {
             const int row = lane / T::CPR + i * (64 / T::CPR);
-            vr[i] = *(const uint4*)(vb + (uint32_t)((full ? row : min(row, last)) * s.row_b + (lane % T::CPR) * 16));
+            vr[i] = *(const uint4*)(vb + (uint32_t)((last >= TK - 1 ? row : min(row, last)) * s.row_b + (lane % T::CPR) * 16));
         }
     }
+    __device__ __forceinline__ void fetch(const KeySegment& s, int t) { fetch_k(s, t); fetch_v(s, t); }
 
     // tiles first, first + 4, ... < s.t1 of a segment; the tile `first` has been requested by fetch()
     __device__ __forceinline__ void run(const KeySegment& s, int first) {
@@ -183,19 +190,6 @@ struct Columns {
     template <bool EDGE>
     __device__ __forceinline__ void tile(const KeySegment& s, int t) {
         const int k0 = t * TK;
-        asm volatile("" ::: "memory");                    // (the previous tile's LDS reads stay in front of these writes: LDS is in order)
-        if (FMT != KV_BF16) sc[lane] = lane < TK ? scr * (A.scale * LOG2E) : scr;
-        bool odd_v = false;                               // a NaN or an infinity in a bf16 V row that some columns must not see
-#pragma unroll
-        for (int i = 0; i < T::VL; ++i) {
-            const int row = lane / T::CPR + i * (64 / T::CPR);
-            *(uint4*)(vimg + row * T::RB + (((lane % T::CPR) ^ T::swz(row)) * 16)) = vr[i];
-            if (FMT == KV_BF16 && EDGE) {
-                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd_v |= amax2(w[e]) >= 0x7f80u;
-            }
-        }
         // ---- S^T = K . Q^T
         f32x4 st[NC][2];
 #pragma unroll
@@ -208,7 +202,7 @@ struct Columns {
                 if (FMT == KV_BF16) kf8[kf] = __builtin_bit_cast(bf16x8, kr[kf][FMT == KV_BF16 ? step : 0]);
                 else {
                     const uint4 x = kr[kf][FMT == KV_BF16 ? 0 : step >> 1];
-                    kf8[kf] = codes_to_bf16<FMT>((step & 1) ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
+                    kf8[kf] = codes_to_bf16<FMT>((step & 1) ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y), kscr[kf]);
                 }
             }
 #pragma unroll
@@ -217,20 +211,37 @@ struct Columns {
                 st[cb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[1], qreg[cb][step], st[cb][1], 0, 0, 0);
             }
         }
-        if (t + 4 < s.t1) fetch(s, t + 4);                // the registers of K and V are free: the next tile is under way during the rest
+        if (t + 4 < s.t1) fetch_k(s, t + 4);              // K's registers are free: the next tile's rows are under way during the rest, V's as soon as
+                                                          // they lie in LDS
+        // ---- V and the scales into the wave's image; (the previous tile's LDS reads stay in front of these writes: LDS is in order)
+        asm volatile("" ::: "memory");
+        if (FMT != KV_BF16) sc[lane] = FMT == KV_INT8 && lane < TK ? scr * (A.scale * LOG2E) : scr;
+        bool odd_v = false;                               // a NaN or an infinity in a bf16 V row that some columns must not see
+#pragma unroll
+        for (int i = 0; i < T::VL; ++i) {
+            const int row = lane / T::CPR + i * (64 / T::CPR);
+            *(uint4*)(vimg + row * T::RB + (((lane % T::CPR) ^ T::swz(row)) * 16)) = vr[i];
+            if (FMT == KV_BF16 && EDGE) {
+                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd_v |= amax2(w[e]) >= 0x7f80u;
+            }
+        }
+        if (t + 4 < s.t1) fetch_v(s, t + 4);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // image and scales complete before any lane reads them
         __builtin_amdgcn_wave_barrier();
-        float ksv[2][4], vsv[2][4];
+        f32x4 ksv[2], vsv[2];
         if (FMT != KV_BF16) {
 #pragma unroll
             for (int kf = 0; kf < 2; ++kf) {
-                const float4 a = *(const float4*)(sc + kf * 16 + g * 4), b = *(const float4*)(sc + TK + kf * 16 + g * 4);
-                ksv[kf][0] = a.x; ksv[kf][1] = a.y; ksv[kf][2] = a.z; ksv[kf][3] = a.w;
-                vsv[kf][0] = b.x; vsv[kf][1] = b.y; vsv[kf][2] = b.z; vsv[kf][3] = b.w;
+                if (FMT == KV_INT8) ksv[kf] = *(const f32x4*)(sc + kf * 16 + g * 4);
+                vsv[kf] = *(const f32x4*)(sc + TK + kf * 16 + g * 4);
             }
         }
         // ---- online softmax in the log2 domain; the running maximum follows only in steps of more than 2^8 (weights stay below 2^8, far
-        //      inside fp32 and bf16), so that O is rescaled a few times per range and not once per tile
+        //      inside fp32 and bf16), so that O is rescaled a few times per range and not once per tile.  x = the score up to the factor kmul > 0,
+        //      which for int8 is in the row scales; elsewhere it is applied by the exponential's fma
+        const float kmul = FMT == KV_INT8 ? 1.f : A.scale * LOG2E;
         bf16x8 pf[NC];
         uint64_t see[NC];
         auto visible = [&](int cb, int key) -> bool { return key < s.base || (key < s.total && ((see[cb] >> (key - s.base)) & 1)); };
@@ -252,12 +263,12 @@ struct Columns {
             for (int kf = 0; kf < 2; ++kf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float x = st[cb][kf][r] * (FMT == KV_BF16 ? A.scale * LOG2E : ksv[kf][r]);
+                    float x = FMT == KV_INT8 ? st[cb][kf][r] * ksv[kf][r] : st[cb][kf][r];
                     if (EDGE && !vis[kf][r]) x = -INFINITY;
                     p[kf][r] = x;
                     mx = fmaxf(mx, x);
                 }
-            mx = group_max(mx);
+            mx = group_max(mx) * kmul;
             if (__any(mx > m_run[cb] + 8.f)) {
                 const float m_new = mx > m_run[cb] + 8.f ? mx : m_run[cb];
                 const float alpha = m_run[cb] == m_new ? 1.f : __builtin_amdgcn_exp2f(m_run[cb] - m_new);
@@ -272,7 +283,7 @@ struct Columns {
             for (int kf = 0; kf < 2; ++kf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[kf][r] = __builtin_amdgcn_exp2f(p[kf][r] - m);
+                    p[kf][r] = __builtin_amdgcn_exp2f(FMT == KV_INT8 ? p[kf][r] - m : fmaf(p[kf][r], kmul, -m));
                     sum += p[kf][r];
                     if (FMT != KV_BF16) {
                         p[kf][r] *= vsv[kf][r];
@@ -321,7 +332,7 @@ struct Columns {
                 typedef __attribute__((ext_vector_type(2))) int i32x2;
                 const int r = l15 >> 1, row = (r >> 2) * 16 + 4 * g + (r & 3);
                 const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(vimg + row * T::RB + ((df ^ T::swz(row)) * 16) + (l15 & 1) * 8));
-                vf = codes_to_bf16<FMT>(make_uint2((uint32_t)x[0], (uint32_t)x[1]));
+                vf = codes_to_bf16<FMT>(make_uint2((uint32_t)x[0], (uint32_t)x[1]), 1.f);
             }
 #pragma unroll
             for (int cb = 0; cb < NC; ++cb) oacc[cb][df] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[cb], oacc[cb][df], 0, 0, 0);
@@ -547,9 +558,9 @@ struct AttnPlan {
 // rollout runs).
 // Short contexts go in one launch: 640 positions, or 1024 where that launch has 128 workgroups or more (one launch | two: 6.3 | 7.6 us at 384
 // positions of 1 x 2 rollouts, 9.5 | 8.7 at 1024; 8 x 8 rollouts 11.1 | 13.4 us at 1024, 15.3 | 14.5 at 1536).
-// Others: of the widths (16 or 32 columns) and numbers of key ranges (sa, sb) the one whose estimate is least.  The estimate's constants (us) were fitted
-// to 1100 launches of 45 shapes (1 to 8 prompts, 1 to 2048 columns, 300 to 14000 positions, all formats): the choice is 4 % behind the best of them in the
-// mean, 8 % with a fixed width of 32.  Two workgroups per CU run at once; a third round rarely ends together with the second.
+// Others: of the widths (16 or 32 columns) and numbers of key ranges (sa, sb) the one whose estimate (us) is least: 512 workgroups run at once (two per CU), one
+// costs a constant and its 32-key tiles per wave, a record of a column its bytes.  The constants were fitted to 2700 launches of 90 settings (1 to 8
+// prompts of equal and of falling lengths, 1 to 2048 columns, 300 to 14000 positions, all formats): the choice is 3 % behind the best of them in the mean.
 AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
     const spacer_kv_cache* c = prompt ? prompt : tail;
     const long rep = Hq / c->kv_heads, cb = N * rep, ca = prompt ? rows * cb : 0, most = ca > cb ? ca : cb;
@@ -563,7 +574,7 @@ AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, i
         return p;
     }
     static const int ranges[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
-    const double start = 36.0, once = 3.8, ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
+    const double once = 5.9, ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
     double best = 1e300;
     for (int nc = 1; nc <= (most > 16 ? 2 : 1); ++nc) {
         const int ncb = cb <= 16 ? 1 : nc, cba = prompt ? cdiv(ca, 16 * nc) : 0, cbb = tail ? cdiv(cb, 16 * ncb) : 0;
@@ -573,11 +584,11 @@ AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, i
             if (ia > 0 && (!prompt || ta < sa)) break;
             for (int sb = tail ? 1 : 0; sb <= (tail ? 4 : 0); sb = sb ? 2 * sb : 1) {
                 if (sb > 1 && tb < sb) break;
-                const double a = sa ? ceil(ta / sa) * (0.21 + 0.155 * nc) : 0, b = sb ? ceil(tb / sb) * (0.21 + 0.155 * ncb) : 0;
-                const double work = 0.5 * start + (ja * sa * (once + a) + jb * sb * (once + b)) / 512, longest = start + (a > b ? a : b);
+                const double a = sa ? ceil(ta / sa) * (0.25 + 0.35 * nc) : 0, b = sb ? ceil(tb / sb) * (0.25 + 0.35 * ncb) : 0;
+                const double work = (ja * sa * (once + a) + jb * sb * (once + b)) / 512, longest = a > b ? a : b;
                 double t = work > longest ? work : longest;
-                if (ja * sa + jb * sb > 512) t += 0.95 * (start + (sa && sb ? (a < b ? a : b) : a + b));
-                t += 2e-4 * p.cols * (sa + sb) + 1.15 * cdiv(sa + sb, 8);
+                if (ja * sa + jb * sb > 512) t += 0.17 * (once + (sa && sb ? (a < b ? a : b) : a + b));
+                t += 0.57e-4 * p.cols * (sa + sb) + 0.53 * cdiv(sa + sb, 8);
                 if (t < best) { best = t; p.nca = nc; p.ncb = ncb; p.cba = cba; p.cbb = cbb; p.sa = sa; p.sb = sb; }
             }
         }
@@ -626,6 +637,7 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
     const spacer_kv_cache* c = prompt ? prompt : tail;
     const int D = c->head_dim, Hkv = c->kv_heads;
     SP_REQUIRE(q && o && (((uintptr_t)q | (uintptr_t)o) & 15) == 0 && q_ld % 8 == 0, SPACER_EINVAL, "attn_cache: q and o rows must start at multiples of 16 bytes");
+    SP_REQUIRE(scale > 0.f && scale < INFINITY, SPACER_EINVAL, "attn_cache: scale %g must be a positive number", (double)scale);
     SP_REQUIRE(!prompt || prompt_len, SPACER_EINVAL, "attn_cache: prompt_len required");
     SP_REQUIRE(!prompt || row0 || (long)prompt->n_seq * rows == B, SPACER_EINVAL, "attn_cache: %d prompts x %d rows, %d sequences", prompt ? prompt->n_seq : 0, rows, B);
     SP_REQUIRE(!tail || tail_len, SPACER_EINVAL, "attn_cache: tail_len required");

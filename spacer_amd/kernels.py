@@ -491,7 +491,7 @@ class KVCache:
     [n_seq, kv_heads, capacity], and stand for code * scale:
         float8_e4m3fn   scale = the smallest power of two >= 2^-126 with max|row| / scale <= 448
         int8            scale = max|row| / 127, codes -127 .. 127, ties of x / scale to even
-    A row that holds a NaN or an infinity gets scale NaN.  The object only describes the tensors (and keeps them alive)."""
+    A row that holds a NaN or an infinity gets scale NaN.  (e4m3 scales made elsewhere must be powers of two too.)  The object only describes the tensors (and keeps them alive)."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "kv_heads", "capacity", "head_dim", "dtype", "device", "_c", "_ref", "_shape")
 
@@ -633,7 +633,7 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
     [B, nodes]; None: node i sees the nodes up to and including itself.  A node that sees nothing gets zeros.
     ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` sequences from
     p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt each.
-    prompt_len int32 [n_prompts]; tail_len int32 [B] or [1].  ``workspace``: attn_cache_workspace_bytes bytes; None allocates it."""
+    prompt_len int32 [n_prompts]; tail_len int32 [B] or [1]; scale > 0.  ``workspace``: attn_cache_workspace_bytes bytes; None allocates it."""
     c = prompt if prompt is not None else tail
     if c is None:
         raise SpacerError("attn_cache: a prompt or a tail cache is needed")

@@ -72,10 +72,10 @@ def test_entries_refuse(lib):
     assert lib.spacer_kv_read(r, None, p, None, 0, None) == EINVAL
     assert lib.spacer_kv_read(r, None, p + 4, p, 0, None) == EINVAL
 
-    def attn(q=p, ld=512, prompt=r, plen=p, row0=None, rows=1, tail=r, tlen=p, o=p, B=2, N=1, Hq=4, ws=p, n=1 << 30):
-        return lib.spacer_attn_cache(q, ld, prompt, plen, row0, rows, tail, tlen, 0, None, 0, o, B, N, Hq, 1.0, ws, n, None)
+    def attn(q=p, ld=512, prompt=r, plen=p, row0=None, rows=1, tail=r, tlen=p, o=p, B=2, N=1, Hq=4, ws=p, n=1 << 30, scale=1.0):
+        return lib.spacer_attn_cache(q, ld, prompt, plen, row0, rows, tail, tlen, 0, None, 0, o, B, N, Hq, scale, ws, n, None)
     for kw in (dict(q=None), dict(q=p + 8), dict(ld=516), dict(prompt=None, tail=None), dict(plen=None), dict(tlen=None), dict(o=None), dict(B=3), dict(B=-1), dict(N=0), dict(N=65),
-               dict(Hq=3), dict(Hq=0), dict(rows=0), dict(rows=2), dict(prompt=C.byref(cache(head_dim=64))), dict(prompt=C.byref(cache(format=1))),
+               dict(Hq=3), dict(Hq=0), dict(rows=0), dict(rows=2), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf")), dict(prompt=C.byref(cache(head_dim=64))), dict(prompt=C.byref(cache(format=1))),
                dict(prompt=C.byref(cache(kv_heads=1)))):
         assert attn(**kw) == EINVAL, kw
     # (short contexts need no workspace)
