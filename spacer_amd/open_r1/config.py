@@ -68,6 +68,9 @@ class GRPOConfig:                              # the trl.GRPOConfig / TrainingAr
     deepspeed: Optional[str] = None
     top_k: int = 50                # era default of the GenerationConfig the reference builds
     use_decode_graph: bool = True
+    # rollouts (SamplingParams): format of the key/value caches (bf16 | e4m3 | int8) and HF's repetition_penalty
+    kv_cache: str = "bf16"
+    repetition_penalty: float = 1.0
     # gradient-accumulation micro-batches scored / back-propagated per token-packed pass (GRPOEngine.score_and_backward_multi);
     # 2 fits 288 GB at 7B with 16-frame prompts and 512-token rollouts, 1 = one prompt group per pass
     groups_per_pass: int = 2

@@ -372,7 +372,8 @@ class SGRLVRTrainer:
         not a second decode loop.  Returns per sample dict(prompt, completion_ids [G, C], shuffled_ids [G/2, C] or None)."""
         G = self.num_generations
         sp = SamplingParams(max_new_tokens=self.max_completion_length, top_k=self.args.top_k, top_p=0.95, temperature=1.0,
-                            seed=self._sample_seed + 7919 * self.global_step, era_rule=self.era_rule, suppress_eos=self.suppress_eos)
+                            seed=self._sample_seed + 7919 * self.global_step, era_rule=self.era_rule, suppress_eos=self.suppress_eos,
+                            kv_cache=self.args.kv_cache, repetition_penalty=self.args.repetition_penalty)
         # batch order: every sample's own prompt first, the frame-shuffled twins behind them -- the scored prompts are then CONSECUTIVE
         # in the prefill pass, which is what lets the policy's scoring pass take its prompt rows from a kept prefill tape
         # (Qwen2VLEngine._prefill_usable; interleaved [p0, twin0, p1, twin1] never qualified with two groups per pass: ADVICE r5)

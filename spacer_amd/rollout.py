@@ -16,7 +16,7 @@ import os
 import weakref
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -77,6 +77,90 @@ class SamplingParams:
     # (L_b > max_new_tokens: no EOS).  EOS is forbidden everywhere else (spacer_eos_schedule on the step's logits), the loop ends
     # when every row has finished, completions are padded behind EOS -- the shape of a real run's batch, with known lengths.
     synthetic_lengths: Optional[Tuple[int, int]] = None
+    # format of the prompts' and the rollouts' key/value caches: "bf16", or one byte per number with a scale per token and head --
+    # "e4m3" / "int8" (kernels.KVCache; half the cache's bytes, decode attention through kernels.attn_cache)
+    kv_cache: str = "bf16"
+    # logits before temperature / top_k / top_p (kernels.process_logits), in this order: HF's repetition_penalty on tokens of the prompt and the
+    # completion; frequency and presence penalties on the completion's tokens; a bias per token id; only these token ids may be drawn
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None
+    allowed_token_ids: Optional[Sequence[int]] = None
+
+
+class _LayerCaches:
+    """One kernels.KVCache per decoder layer over common allocations [layers, n_seq, kv_heads, capacity, head_dim]."""
+
+    def __init__(self, layers: int, n_seq: int, capacity: int, kv_heads: int, head_dim: int, dtype: str, device):
+        self.codes = [torch.zeros(layers, n_seq, kv_heads, capacity, head_dim, device=device, dtype=torch.uint8).view(K.KV_DTYPES[dtype]) for _ in range(2)]
+        self.scales = [torch.zeros(layers, n_seq, kv_heads, capacity, device=device, dtype=F32) for _ in range(2)]
+        self.layers = [self.part(i, 0, n_seq) for i in range(layers)]
+        self.capacity = capacity
+
+    def part(self, layer: int, a: int, b: int) -> K.KVCache:
+        """Sequences [a, b) of a layer."""
+        (k, v), (ks, vs) = ((x[layer][a:b] for x in pair) for pair in (self.codes, self.scales))
+        return K.KVCache(k, v, ks, vs)
+
+
+class _LogitRules:
+    """What ``SamplingParams`` asks of the logits before the sampler, for ``B`` rows of one generate call: the tokens' history and the tables
+    live on the device, so that a captured decode step carries them on."""
+
+    def __init__(self, sp: SamplingParams, prompts, counts: Sequence[int], vocab: int, eos_id: int, device):
+        B = sum(counts)
+        bias = None
+        if sp.logit_bias:
+            bias = torch.zeros(vocab, dtype=F32)
+            for token, value in sp.logit_bias.items():
+                token, value = int(token), float(value)
+                if not 0 <= token < vocab or value != value or value == float("inf"):
+                    raise ValueError(f"SamplingParams.logit_bias: token {token} (vocabulary {vocab}), value {value}")
+                bias[token] = value
+        allowed = torch.ones(vocab, dtype=torch.bool)
+        if sp.allowed_token_ids is not None:
+            ids = torch.tensor([int(i) for i in sp.allowed_token_ids], dtype=torch.int64)
+            if ids.numel() == 0 or int(ids.min()) < 0 or int(ids.max()) >= vocab:
+                raise ValueError("SamplingParams.allowed_token_ids: an empty list, or ids outside the vocabulary")
+            allowed = torch.zeros(vocab, dtype=torch.bool)
+            allowed[ids] = True
+        drawable = allowed.clone() if bias is None else allowed & (bias > float("-inf"))
+        if sp.suppress_eos:
+            drawable[eos_id] = False
+        if not bool(drawable.any()):
+            raise ValueError("SamplingParams: allowed_token_ids, logit_bias and suppress_eos leave no token to draw")
+        self.penalties = dict(repetition=float(sp.repetition_penalty), frequency=float(sp.frequency_penalty), presence=float(sp.presence_penalty))
+        if not 0.0 < self.penalties["repetition"] < float("inf") or any(not abs(self.penalties[n]) < float("inf") for n in ("frequency", "presence")):
+            raise ValueError(f"SamplingParams: penalties {self.penalties}: finite numbers, the repetition penalty above 0")
+        self.bias = None if bias is None else bias.to(device)
+        self.allowed = None
+        if sp.allowed_token_ids is not None:
+            wide = torch.zeros((vocab + 31) // 32 * 32, dtype=torch.int64)
+            wide[:vocab] = allowed
+            words = (wide.view(-1, 32) << torch.arange(32)).sum(-1)
+            self.allowed = torch.where(words >= 2 ** 31, words - 2 ** 32, words).int()[None].to(device)
+        self.seen = self.counts = None
+        if self.penalties != dict(repetition=1.0, frequency=0.0, presence=0.0):
+            self.seen, self.counts = K.token_history(B, vocab, device)
+            row = 0
+            for pr, k in zip(prompts, counts):
+                K.token_history_add_(self.seen[row:row + k], None, pr.ids.expand(k, -1), vocab=vocab)
+                row += k
+        self.vocab = vocab
+
+    @staticmethod
+    def wanted(sp: SamplingParams) -> bool:
+        return bool(sp.repetition_penalty != 1.0 or sp.frequency_penalty or sp.presence_penalty or sp.logit_bias or sp.allowed_token_ids is not None)
+
+    def add(self, ids: torch.Tensor) -> None:
+        """The tokens that the rows drew last (int64 [B]); a finished row's padding counts too and is never read."""
+        if self.seen is not None:
+            K.token_history_add_(self.seen, self.counts, ids[:, None], vocab=self.vocab)
+
+    def apply(self, logits: torch.Tensor) -> None:
+        penalties = self.penalties if self.seen is not None else {}
+        K.process_logits(logits, seen=self.seen, counts=self.counts, bias=self.bias, allowed=self.allowed, **penalties)
 
 
 class RolloutEngine:
@@ -190,7 +274,7 @@ class RolloutEngine:
         with M = total prompt tokens): the reference runs this per rollout inside HF generate (TR:463).  ``keep_tape``: the pass
         is taped like a scoring pass and every prompt receives its ``PrefillSlice``.  ``out`` = (pk, pv, p0): write the prompt KV of
         these prompts into slots [p0, p0 + len(prompts)) of caches allocated by the caller (a taped and an untaped pass over two
-        parts of the batch share one cache)."""
+        parts of the batch share one cache); pk may also be a ``_LayerCaches`` (then pv is None)."""
         cfg, e = self.cfg, self.e
         L, Hkv, D = cfg.layers, cfg.kv_heads, cfg.head_dim
         nP = len(prompts)
@@ -202,12 +286,15 @@ class RolloutEngine:
             Pmax = max(plen)
             pk = torch.empty(L, nP, Pmax, Hkv, D, device=self.dev, dtype=BF16)
             pv = torch.empty_like(pk)
+        elif isinstance(out[0], _LayerCaches):
+            pk, pv = out[0], None
+            Pmax = pk.capacity
         else:
             pk, pv = out[0][:, out[2]:out[2] + nP], out[1][:, out[2]:out[2] + nP]        # [L, nP, Pmax, Hkv, D] views
             Pmax = pk.shape[2]
         # packed row of every (prompt, position) slot of the prompt KV cache; slots past a prompt's length are never read
-        # (the attention kernels stop at plen) and take row 0
-        gidx = torch.zeros(nP, Pmax, dtype=torch.int32)
+        # (the attention kernels stop at plen) and take row 0; of an 8-bit cache they are left alone
+        gidx = torch.full((nP, Pmax), -1 if isinstance(pk, _LayerCaches) else 0, dtype=torch.int32)
         for pi, (s0, P) in enumerate(zip(starts, plen)):
             gidx[pi, :P] = torch.arange(s0, s0 + P, dtype=torch.int32)
         gidx = gidx.reshape(-1).to(self.dev)
@@ -228,6 +315,9 @@ class RolloutEngine:
         segs = K.make_segments([(s0, P, 0, 0) for s0, P in zip(starts, plen)], self.dev)
 
         def sink(layer, k, v):          # one row gather per tensor per layer (was one device copy per prompt)
+            if isinstance(pk, _LayerCaches):
+                K.kv_write(pk.part(layer, out[2], out[2] + nP), k, v, gidx)
+                return
             K.gather_rows(k, gidx, out=pk[layer].view(nP * Pmax, Hkv * D))
             K.gather_rows(v, gidx, out=pv[layer].view(nP * Pmax, Hkv * D))
 
@@ -262,14 +352,24 @@ class RolloutEngine:
                 # finishing kernel applies rstd (and clears the next layer's row sums)
                 rs = st["rowss"]
                 K.gemm_skinny_packed_normed(x, PW[p + "qkv_wn"], st["acc_qkv"], rs[i], cfg.qkv_dim)
-                K.decode_qkv_finish_normed(st["acc_qkv"], W[p + "qkv_b"], st["cos"], st["sin"], st["q"], st["tk"][i], st["tv"][i],
-                                           st["tail_len"], rs[i], rs[(i + 1) % cfg.layers], cfg.hidden, cfg.rms_eps, Hq, Hkv, D)
+                if st["tail"] is not None:
+                    K.decode_qkv_finish_cache(st["acc_qkv"], W[p + "qkv_b"], st["cos"], st["sin"], st["q"], st["tail"].layers[i], st["tail_len"], Hq,
+                                              rowss=rs[i], rowss_zero=rs[(i + 1) % cfg.layers], norm_cols=cfg.hidden, eps=cfg.rms_eps)
+                else:
+                    K.decode_qkv_finish_normed(st["acc_qkv"], W[p + "qkv_b"], st["cos"], st["sin"], st["q"], st["tk"][i], st["tv"][i],
+                                               st["tail_len"], rs[i], rs[(i + 1) % cfg.layers], cfg.hidden, cfg.rms_eps, Hq, Hkv, D)
             else:
                 h = K.rmsnorm_fwd(x, W[p + "ln1_w"], cfg.rms_eps, out=st["h"])
                 K.gemm_skinny_packed_acc(h, PW[p + "qkv_w"], st["acc_qkv"], cfg.qkv_dim)
-                K.decode_qkv_finish(st["acc_qkv"], W[p + "qkv_b"], st["cos"], st["sin"], st["q"], st["tk"][i], st["tv"][i],
-                                    st["tail_len"], Hq, Hkv, D)
-            if st["shared_prefix"] and st["row0"] is not None:      # ... with per-prompt rollout counts (the T-GRPO twins: G / 2)
+                if st["tail"] is not None:
+                    K.decode_qkv_finish_cache(st["acc_qkv"], W[p + "qkv_b"], st["cos"], st["sin"], st["q"], st["tail"].layers[i], st["tail_len"], Hq)
+                else:
+                    K.decode_qkv_finish(st["acc_qkv"], W[p + "qkv_b"], st["cos"], st["sin"], st["q"], st["tk"][i], st["tv"][i],
+                                        st["tail_len"], Hq, Hkv, D)
+            if st["tail"] is not None:       # 8-bit caches: any number of rows per prompt
+                o = K.attn_cache(st["q"], st["pk"].layers[i], st["plen"], st["tail"].layers[i], st["tail_len"], Hq, scale, rows_per_prompt=st["Kn"],
+                                 row0=st["row0"], out=st["o"], workspace=st["attn_ws"])
+            elif st["shared_prefix"] and st["row0"] is not None:      # ... with per-prompt rollout counts (the T-GRPO twins: G / 2)
                 o = K.attn_decode_shared_rows(st["q"], st["pk"][i], st["pv"][i], st["plen"], st["prompt_of"], st["row0"], st["tk"][i],
                                               st["tv"][i], st["tail_len"], st["Kn"], Hq, Hkv, D, scale, out=st["o"], workspace=st["attn_ws"])
             elif st["shared_prefix"]:      # prompt keys scored once per prompt for its K rollouts
@@ -291,6 +391,9 @@ class RolloutEngine:
         else:
             st["logits"].zero_()
             K.gemm_skinny_packed_acc(hn, PW["llm.lm_head"], st["logits"], cfg.vocab)
+        if st["rules"] is not None:                      # (cur_tok is the token that this step's rows drew last)
+            st["rules"].add(st["cur_tok"])
+            st["rules"].apply(st["logits"])
         if st.get("eos_at") is not None:                 # synthetic lengths: EOS only at the scheduled token index of each row
             K.eos_schedule_(st["logits"], st["step"], 1, st["eos_at"], cfg.eos_token_id)
         # Philox step / output column = counter + 1 = index of the token being drawn
@@ -339,6 +442,9 @@ class RolloutEngine:
                 a, r0 = b, r0 + rows
             return torch.cat(outs, 0)
         dev = self.dev
+        if sp.kv_cache not in K.KV_DTYPES:
+            raise ValueError(f"SamplingParams.kv_cache: {sp.kv_cache!r} (one of {sorted(K.KV_DTYPES)})")
+        rules = _LogitRules(sp, prompts, counts, cfg.vocab, cfg.eos_token_id, dev) if _LogitRules.wanted(sp) else None
         ev = [torch.cuda.Event(enable_timing=True) for _ in range(3)] if stats is not None else None
         if ev:
             ev[0].record()
@@ -353,13 +459,14 @@ class RolloutEngine:
         if n_keep == 0:
             self.prefill_tape_bytes = 0
         self.prefill_tape_prompts = n_keep               # (of len(prompts), counted from the front)
+        narrow = None if sp.kv_cache == "bf16" else _LayerCaches(cfg.layers, nP, max(p.ids.numel() for p in prompts), cfg.kv_heads, cfg.head_dim, sp.kv_cache, dev)
         if n_keep in (0, len(prompts)):
-            pk, pv, first_logits, plen, pos_base = self._prefill(prompts, sp.era_rule, keep_tape=n_keep > 0)
+            pk, pv, first_logits, plen, pos_base = self._prefill(prompts, sp.era_rule, keep_tape=n_keep > 0, out=None if narrow is None else (narrow, None, 0))
         else:
             # the first n_keep prompts as a taped pass, the others as an untaped one, into one prompt-KV cache
             Pmax_all = max(p.ids.numel() for p in prompts)
-            pk = torch.empty(cfg.layers, len(prompts), Pmax_all, cfg.kv_heads, cfg.head_dim, device=dev, dtype=BF16)
-            pv = torch.empty_like(pk)
+            pk = narrow if narrow is not None else torch.empty(cfg.layers, len(prompts), Pmax_all, cfg.kv_heads, cfg.head_dim, device=dev, dtype=BF16)
+            pv = torch.empty_like(pk) if narrow is None else None
             _, _, fl_a, plen_a, pb_a = self._prefill(prompts[:n_keep], sp.era_rule, keep_tape=True, out=(pk, pv, 0))
             _, _, fl_b, plen_b, pb_b = self._prefill(prompts[n_keep:], sp.era_rule, keep_tape=False, out=(pk, pv, n_keep))
             first_logits, plen, pos_base = torch.cat([fl_a, fl_b], 0), plen_a + plen_b, pb_a + pb_b
@@ -369,11 +476,13 @@ class RolloutEngine:
         st = dict(
             B=B, pk=pk, pv=pv, packed=self._pack(B), Kn=Kn, shared_prefix=Kn * (cfg.heads // cfg.kv_heads) <= 64 and Kn > 1 and not (DECODE_SMALL_ATTN1 and B <= 16),
             row0=None if uniform else torch.tensor([sum(counts[:i]) for i in range(nP + 1)], dtype=torch.int32, device=dev),
-            attn_ws=torch.empty(K.attn_decode_workspace_bytes(nP, cfg.kv_heads) // 4, device=dev, dtype=F32),
+            attn_ws=torch.empty(K.attn_decode_workspace_bytes(nP, cfg.kv_heads) // 4, device=dev, dtype=F32) if narrow is None else None,
             plen=torch.tensor(plen, dtype=torch.int32, device=dev),
             prompt_of=torch.repeat_interleave(torch.arange(nP, dtype=torch.int32), torch.tensor(counts)).to(dev),
             pos_base=torch.repeat_interleave(torch.tensor(pos_base, dtype=torch.int32), torch.tensor(counts)).to(dev).contiguous(),
-            tk=K.zeros(L, B, C, Hkv, D, device=dev, dtype=BF16), tv=K.zeros(L, B, C, Hkv, D, device=dev, dtype=BF16),
+            tk=K.zeros(L, B, C, Hkv, D, device=dev, dtype=BF16) if narrow is None else None,
+            tv=K.zeros(L, B, C, Hkv, D, device=dev, dtype=BF16) if narrow is None else None,
+            tail=None if narrow is None else _LayerCaches(L, B, C, Hkv, D, sp.kv_cache, dev), rules=rules,
             tail_len=torch.full((1,), -1, dtype=torch.int32, device=dev), step=torch.full((1,), -1, dtype=torch.int32, device=dev),
             finished=torch.zeros(B, dtype=torch.int32, device=dev), cur_tok=torch.empty(B, dtype=torch.int64, device=dev),
             x=torch.empty(B, H, device=dev, dtype=F32), h=torch.empty(B, H, device=dev, dtype=BF16),
@@ -385,12 +494,17 @@ class RolloutEngine:
             logits=torch.empty(B, cfg.vocab, device=dev, dtype=F32),
             sample_ws=K.sample_workspace(B, cfg.vocab, dev) if SAMPLER_WIDE else None,
         )
+        if narrow is not None:
+            n = K.attn_cache_workspace_bytes(narrow.layers[0], st["tail"].layers[0], Kn, B, 1, cfg.heads)
+            st["attn_ws"] = torch.empty(n, device=dev, dtype=torch.uint8)
         out = st["out"] = torch.full((B, C), cfg.pad_token_id, dtype=torch.int64, device=dev)
         st["eos_at"] = None if _eos_at is None else _eos_at.to(dev)
         if st["eos_at"] is not None and sp.suppress_eos:
             raise ValueError("SamplingParams: synthetic_lengths schedules EOS itself; suppress_eos must be False")
         # token 0 of every rollout comes from the prompt's last-position logits (K independent draws per prompt)
         st["logits"].copy_(first_logits.index_select(0, st["prompt_of"].long()))
+        if rules is not None:
+            rules.apply(st["logits"])
         if st["eos_at"] is not None:
             K.eos_schedule_(st["logits"], st["step"], 1, st["eos_at"], cfg.eos_token_id)
         K.sample_top_p_step(st["logits"], st["step"], 1, out, top_k=sp.top_k, top_p=sp.top_p, temperature=sp.temperature, seed=sp.seed,
