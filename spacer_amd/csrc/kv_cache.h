@@ -45,6 +45,14 @@ struct RowScale {
     bool finite;
 };
 
+// a / 127 rounded to nearest: the product with the rounded 1 / 127 and one step with its exact remainder (equal to the division for every finite bf16 a
+// of 2^-96 and more; below, the division itself)
+__device__ __forceinline__ float div127(float a) {
+    if (a < 1.2621774e-29f) return a / 127.f;
+    const float c = 1.f / 127.f, y = a * c;
+    return fmaf(fmaf(-127.f, y, a), c, y);
+}
+
 // amax as the bits of |bf16|: NaN > infinity > every finite value, so one integer maximum finds both
 template <int FMT>
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
@@ -59,7 +67,7 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
         r.inv = __uint_as_float((uint32_t)(254 - b) << 23);
     } else {
         const float amax = __uint_as_float(amax_bits << 16);
-        r.scale = r.finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
+        r.scale = r.finite ? div127(amax) : __uint_as_float(0x7fc00000u);
         if (amax < 1.2621774e-29f) r.pre = 18446744073709551616.f;      // 2^-96, 2^64: keeps 1 / s finite
         r.s = r.scale * r.pre;
         r.inv = (r.finite && r.s > 0.f) ? 1.f / r.s : 0.f;
@@ -85,6 +93,49 @@ __device__ __forceinline__ uint32_t code2(uint32_t w, const RowScale& r) {
     if (FMT == KV_E4M3) return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * r.inv, b * r.inv, 0, false) & 0xffffu;
     if (r.inv == 0.f) return 0u;
     return ((uint32_t)(int)quotient_rne(a, r) & 0xffu) | (((uint32_t)(int)quotient_rne(b, r) & 0xffu) << 8);
+}
+
+// What the eight-code form below needs of an int8 row.  1 / s comes from the hardware reciprocal (1 ulp) and is moved by at most 4 ulp so that max|x| / 2, which
+// every other wave holds and whose quotient 63.5 (1 + error of s) lies next to a half, falls on the side of 63.5 that the exact quotient lies on (a
+// tie's even neighbour is 64, outside).  Other numbers next to a half go the exact way.
+struct Int8Row {
+    float inv;
+    uint32_t half;       // max|x| / 2 as bf16 bits
+    bool exact;          // tiny, zero or non-finite row
+};
+__device__ __forceinline__ Int8Row int8_row(const RowScale& r, uint32_t amax_bits) {
+    Int8Row q;
+    const float amax = __uint_as_float(amax_bits << 16), inv = __builtin_amdgcn_rcpf(r.scale);
+    const bool outside = fmaf(-127.f, r.scale, amax) >= 0.f, is = fmaf(amax, inv, -127.f) >= 0.f;
+    q.inv = __uint_as_float(__float_as_uint(inv) + (outside == is ? 0 : outside ? 4 : -4));
+    q.half = amax_bits - (1u << 7);
+    q.exact = amax_bits < (31u << 7) || !r.finite;                                  // (31 << 7: 2^-96)
+    return q;
+}
+// Eight int8 codes: u = x (1 / s) + 1.5 2^23 rounds the product to an integer in u's low bits.  1 / s is off by less than 5 2^-23 of itself, so the product
+// by less than 7.6e-5: the integer is the right one where the product is further than 1e-4 from a half.  A wave that holds another number there (one in
+// ten) or an exact row takes the comparison of quotient_rne for all.
+__device__ __forceinline__ uint2 codes8_int8(const uint4 x, const RowScale& r, const Int8Row& q) {
+    const float magic = 12582912.f;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float u[8], far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = (i & 1) ? bf_hi(w[i >> 1]) : bf_lo(w[i >> 1]);
+        u[i] = fmaf(f, q.inv, magic);
+        const float off = fmaf(f, q.inv, magic - u[i]);
+        far = fmaxf(far, fabsf(f) == __uint_as_float(q.half << 16) ? 0.f : fabsf(off));
+    }
+    if (__any(q.exact || !(far < 0.4999f)))
+        return make_uint2(code2<KV_INT8>(x.x, r) | (code2<KV_INT8>(x.y, r) << 16), code2<KV_INT8>(x.z, r) | (code2<KV_INT8>(x.w, r) << 16));
+    uint32_t o[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(u[4 * i + 1]), __float_as_uint(u[4 * i]), 0x0c0c0400u);
+        const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(u[4 * i + 3]), __float_as_uint(u[4 * i + 2]), 0x04000c0cu);
+        o[i] = ab | cd;
+    }
+    return make_uint2(o[0], o[1]);
 }
 
 __device__ __forceinline__ uint32_t amax2(uint32_t w) { return max(w & 0x7fffu, (w >> 16) & 0x7fffu); }

@@ -10,74 +10,94 @@
 
 namespace {
 
-template <int FMT, int D>
-__device__ __forceinline__ void store_row(char* dst, float* scale, const uint4 x, int lane_in_row) {
-    constexpr int LPR = D / 8;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+__device__ __forceinline__ u16x2 max2(u16x2 a, u16x2 b) { return __builtin_elementwise_max(a, b); }
+template <int CTRL>
+__device__ __forceinline__ u16x2 max_dpp(u16x2 x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return max2(x, __builtin_bit_cast(u16x2, (uint32_t)__builtin_amdgcn_update_dpp((int)u, (int)u, CTRL, 0xf, 0xf, true)));
+}
+// (max |k|, max |v|) of a row's 8 or 16 lanes, as the bits of |bf16|: packed 16-bit maxima, lanes exchanged by DPP (pairs, quads, halves, rows)
+template <int LPR>
+__device__ __forceinline__ u16x2 row_amax(const uint4 k, const uint4 v) {
+    auto abs2 = [](uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
+    const u16x2 a = max2(max2(abs2(k.x), abs2(k.y)), max2(abs2(k.z), abs2(k.w))), b = max2(max2(abs2(v.x), abs2(v.y)), max2(abs2(v.z), abs2(v.w)));
+    u16x2 m = max2((u16x2){a[0], b[0]}, (u16x2){a[1], b[1]});
+    m = max_dpp<0xb1>(m);
+    m = max_dpp<0x4e>(m);
+    m = max_dpp<0x141>(m);
+    if (LPR == 16) m = max_dpp<0x140>(m);
+    return m;
+}
+
+template <int FMT>
+__device__ __forceinline__ void store_row(char* dst, float* scale, const uint4 x, uint32_t amax, int lane_in_row) {
     if (FMT == KV_BF16) {
         *(uint4*)(dst + lane_in_row * 16) = x;
         return;
     }
-    uint32_t a = max(max(amax2(x.x), amax2(x.y)), max(amax2(x.z), amax2(x.w)));
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
-    const RowScale r = row_scale<FMT>(a);
-    const uint32_t lo = code2<FMT>(x.x, r) | (code2<FMT>(x.y, r) << 16), hi = code2<FMT>(x.z, r) | (code2<FMT>(x.w, r) << 16);
-    *(uint2*)(dst + lane_in_row * 8) = make_uint2(lo, hi);
+    const RowScale r = row_scale<FMT>(amax);
+    *(uint2*)(dst + lane_in_row * 8) = FMT == KV_INT8 ? codes8_int8(x, r, int8_row(r, amax))
+        : make_uint2(code2<FMT>(x.x, r) | (code2<FMT>(x.y, r) << 16), code2<FMT>(x.z, r) | (code2<FMT>(x.w, r) << 16));
     if (lane_in_row == 0) *scale = r.scale;
 }
 
 // Rows of a pass: sequence (blockIdx.x / chunks, a scalar), then row = position * Hkv + head inside it (32 bits), so that the heads of a token,
-// side by side in the source, fall to one wave.  A lane holds a piece of RU rows at once: their loads are in flight together.
-constexpr int RU = 1;
-template <int D> constexpr int rows_per_step() { return 4 * (512 / D) * RU; }      // rows that a workgroup takes at once
+// side by side in the source, fall to one wave.  A lane holds a piece of RU rows of K and V: all loads are in flight before the first use, without a
+// branch between them (rows that are not stored read row 0).
+constexpr int RU = 2;
+template <int D> constexpr int rows_per_block() { return 4 * (512 / D) * RU; }
 
 // APPEND == false: slot (sequence, position) takes source row rows[slot] (below 0, or >= n_src: the slot stays as it is)
 // APPEND == true : source row sequence * N + i goes to position len[sequence] + i (outside the cache: dropped)
 template <int FMT, int D, bool APPEND>
 __global__ __launch_bounds__(256) void kv_store_kernel(const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, long ld, int n_src,
                                                        const int* __restrict__ rows, const int* __restrict__ len, int len_stride, int N,
-                                                       KvView c, unsigned Hkv, unsigned chunks, unsigned steps) {
+                                                       KvView c, unsigned Hkv, unsigned chunks) {
     constexpr int LPR = D / 8, RPW = 64 / LPR;       // lanes per row, rows per wave
     const int lane = threadIdx.x & 63, lr = lane % LPR;
     const unsigned seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const unsigned total = (unsigned)(APPEND ? N : c.cap) * Hkv;
-    const long first = APPEND ? (long)len[(long)seq * len_stride] : 0;
-    for (unsigned step = 0; step < steps; ++step) {
-        const unsigned r0 = (chunk * steps + step) * rows_per_step<D>() + (threadIdx.x >> 6) * (RPW * RU) + lane / LPR;
-        int pos[RU], h[RU];
-        long src[RU];
+    const unsigned r0 = chunk * rows_per_block<D>() + (threadIdx.x >> 6) * (RPW * RU) + lane / LPR;
+    int pos[RU], h[RU];
+    long src[RU];
+    if (APPEND) {
+        const long first = (long)len[(long)seq * len_stride];
+#pragma unroll
+        for (int u = 0; u < RU; ++u) {
+            const unsigned r = r0 + u * RPW, i = r / Hkv;
+            const long p = first + i;
+            h[u] = (int)(r - i * Hkv);
+            pos[u] = (int)p;
+            src[u] = r < total && p >= 0 && p < c.cap ? (long)seq * N + i : -1;
+        }
+    } else {
+        int at[RU];
 #pragma unroll
         for (int u = 0; u < RU; ++u) {
             const unsigned r = r0 + u * RPW, i = r / Hkv;
             h[u] = (int)(r - i * Hkv);
-            src[u] = -1;
-            if (r < total) {
-                if (APPEND) {
-                    const long p = first + i;
-                    pos[u] = (int)p;
-                    if (p >= 0 && p < c.cap) src[u] = (long)seq * N + i;
-                } else {
-                    pos[u] = (int)i;
-                    src[u] = rows[(long)seq * c.cap + i];
-                    if (src[u] >= n_src) src[u] = -1;
-                }
-            }
+            pos[u] = (int)i;
+            at[u] = rows[(long)seq * c.cap + min(i, (unsigned)c.cap - 1)];
         }
-        uint4 xk[RU], xv[RU];
 #pragma unroll
-        for (int u = 0; u < RU; ++u)
-            if (src[u] >= 0) {                           // (the lanes of a row drop out together)
-                xk[u] = *(const uint4*)(k + src[u] * ld + h[u] * D + lr * 8);
-                xv[u] = *(const uint4*)(v + src[u] * ld + h[u] * D + lr * 8);
-            }
+        for (int u = 0; u < RU; ++u) src[u] = r0 + u * RPW < total && at[u] < n_src ? at[u] : -1;
+    }
+    uint4 xk[RU], xv[RU];
 #pragma unroll
-        for (int u = 0; u < RU; ++u)
-            if (src[u] >= 0) {
-                const long at = (seq * c.s_seq + h[u] * c.s_head + pos[u] * c.s_pos) * kv_size<FMT>();
-                const long sat = seq * c.c_seq + h[u] * c.c_head + pos[u] * c.c_pos;
-                store_row<FMT, D>(c.k + at, c.ks + sat, xk[u], lr);
-                store_row<FMT, D>(c.v + at, c.vs + sat, xv[u], lr);
-            }
+    for (int u = 0; u < RU; ++u) {
+        const long o = max(src[u], 0L) * ld + h[u] * D + lr * 8;
+        xk[u] = *(const uint4*)(k + o);
+        xv[u] = *(const uint4*)(v + o);
+    }
+#pragma unroll
+    for (int u = 0; u < RU; ++u) {
+        const u16x2 top = FMT == KV_BF16 ? (u16x2){0, 0} : row_amax<LPR>(xk[u], xv[u]);
+        if (src[u] < 0) continue;
+        const long at = (seq * c.s_seq + h[u] * c.s_head + pos[u] * c.s_pos) * kv_size<FMT>();
+        const long sat = seq * c.c_seq + h[u] * c.c_head + pos[u] * c.c_pos;
+        store_row<FMT>(c.k + at, c.ks + sat, xk[u], top[0], lr);
+        store_row<FMT>(c.v + at, c.vs + sat, xv[u], top[1], lr);
     }
 }
 
@@ -106,7 +126,6 @@ __device__ __forceinline__ void values8(const char* p, float s, float (&f)[8]) {
     for (int i = 0; i < 8; ++i) f[i] *= s;
 }
 
-constexpr int RD = 2;
 template <int FMT, int D, bool F32>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvView c, const int* __restrict__ len, void* __restrict__ ko, void* __restrict__ vo,
                                                       unsigned Hkv, unsigned chunks) {
@@ -114,24 +133,25 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvView c, const int* __res
     const int lane = threadIdx.x & 63, lr = lane % LPR;
     const unsigned seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const unsigned total = (unsigned)c.cap * Hkv;
-    const unsigned r0 = chunk * (4 * RPW * RD) + (threadIdx.x >> 6) * (RPW * RD) + lane / LPR;
+    const unsigned r0 = chunk * rows_per_block<D>() + (threadIdx.x >> 6) * (RPW * RU) + lane / LPR;
     const int n = len ? len[seq] : c.cap;
-    float a[RD][8], b[RD][8];
+    float a[RU][8], b[RU][8], sk[RU], sv[RU];
 #pragma unroll
-    for (int u = 0; u < RD; ++u) {
-        const unsigned r = r0 + u * RPW, i = r / Hkv, h = r - i * Hkv;
+    for (int u = 0; u < RU; ++u) {
+        const unsigned r = min(r0 + u * RPW, total - 1), i = r / Hkv, h = r - i * Hkv;
+        const long sat = seq * c.c_seq + h * c.c_head + i * c.c_pos;
+        sk[u] = FMT == KV_BF16 ? 1.f : c.ks[sat];
+        sv[u] = FMT == KV_BF16 ? 1.f : c.vs[sat];
+        const long at = (seq * c.s_seq + h * c.s_head + i * c.s_pos + lr * 8) * kv_size<FMT>();
+        values8<FMT>(c.k + at, sk[u], a[u]);
+        values8<FMT>(c.v + at, sv[u], b[u]);
+        if ((int)i >= n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[u][e] = b[u][e] = 0.f;
-        if (r < total && (int)i < n) {
-            const long at = (seq * c.s_seq + h * c.s_head + i * c.s_pos + lr * 8) * kv_size<FMT>();
-            const long sat = seq * c.c_seq + h * c.c_head + i * c.c_pos;
-            const float sk = FMT == KV_BF16 ? 1.f : c.ks[sat], sv = FMT == KV_BF16 ? 1.f : c.vs[sat];
-            values8<FMT>(c.k + at, sk, a[u]);
-            values8<FMT>(c.v + at, sv, b[u]);
+            for (int e = 0; e < 8; ++e) a[u][e] = b[u][e] = 0.f;
         }
     }
 #pragma unroll
-    for (int u = 0; u < RD; ++u) {
+    for (int u = 0; u < RU; ++u) {
         const unsigned r = r0 + u * RPW;
         if (r >= total) continue;
         const long o = ((long)seq * total + r) * D + lr * 8;
@@ -232,10 +252,6 @@ static unsigned row_chunks(long n_seq, long rows, int per) {
     const long chunks = (rows + per - 1) / per;
     return rows < 0x7fffffffL - 4096 && n_seq * chunks <= 0x7fffffffL ? (unsigned)chunks : 0u;
 }
-// A workgroup takes 4 steps where that still leaves two workgroups per CU: the scales of neighbouring positions (4 bytes each) then leave one
-// workgroup, i.e. one XCD's L2, as whole lines.
-static unsigned store_steps(long n_seq, long rows, int D) { return 1; }
-
 static int check_source(const void* k, const void* v, long ld, const char* who) {
     SP_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ld % 8 == 0, SPACER_EINVAL, "%s: source rows must start at multiples of 16 bytes", who);
     return SPACER_OK;
@@ -247,11 +263,11 @@ extern "C" int spacer_kv_write(const spacer_kv_cache* c, const void* k, const vo
     if (n_src == 0) return SPACER_OK;
     if (int rc = check_source(k, v, ld, "kv_write")) return rc;
     const long per_seq = (long)c->capacity * c->kv_heads;
-    const unsigned steps = store_steps(c->n_seq, per_seq, c->head_dim), chunks = row_chunks(c->n_seq, per_seq, steps * 4 * (512 / c->head_dim) * RU);
+    const unsigned chunks = row_chunks(c->n_seq, per_seq, 4 * (512 / c->head_dim) * RU);
     SP_REQUIRE(chunks, SPACER_EINVAL, "kv_write: cache too large");
 #define CALL(F, D)                                                                                                                                   \
     hipLaunchKernelGGL((kv_store_kernel<F, D, false>), dim3(c->n_seq * chunks), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
-                       ld, n_src, rows, (const int*)nullptr, 0, 1, spacer_kv_view(c), c->kv_heads, chunks, steps)
+                       ld, n_src, rows, (const int*)nullptr, 0, 1, spacer_kv_view(c), c->kv_heads, chunks)
     KV_DISPATCH(c, CALL);
 #undef CALL
     SP_CHECK_LAUNCH();
@@ -265,11 +281,11 @@ extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const v
     if (N == 0) return SPACER_OK;
     if (int rc = check_source(k, v, ld, "kv_append")) return rc;
     const long per_seq = (long)N * c->kv_heads;
-    const unsigned steps = store_steps(c->n_seq, per_seq, c->head_dim), chunks = row_chunks(c->n_seq, per_seq, steps * 4 * (512 / c->head_dim) * RU);
+    const unsigned chunks = row_chunks(c->n_seq, per_seq, 4 * (512 / c->head_dim) * RU);
     SP_REQUIRE(chunks && (long)c->n_seq * N <= 0x7fffffffL, SPACER_EINVAL, "kv_append: %d sequences x %d tokens are too many", c->n_seq, N);
 #define CALL(F, D)                                                                                                                                  \
     hipLaunchKernelGGL((kv_store_kernel<F, D, true>), dim3(c->n_seq * chunks), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k, (const bf16_t*)v, \
-                       ld, c->n_seq * N, (const int*)nullptr, len, len_per_seq ? 1 : 0, N, spacer_kv_view(c), c->kv_heads, chunks, steps)
+                       ld, c->n_seq * N, (const int*)nullptr, len, len_per_seq ? 1 : 0, N, spacer_kv_view(c), c->kv_heads, chunks)
     KV_DISPATCH(c, CALL);
 #undef CALL
     SP_CHECK_LAUNCH();
@@ -279,7 +295,7 @@ extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const v
 extern "C" int spacer_kv_read(const spacer_kv_cache* c, const int* len, void* k_out, void* v_out, int out_f32, spacer_stream_t stream) {
     if (int rc = spacer_check_kv_cache(c, "kv_read")) return rc;
     SP_REQUIRE(k_out && v_out && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, SPACER_EINVAL, "kv_read: outputs must be 16-byte aligned");
-    const unsigned chunks = row_chunks(c->n_seq, (long)c->capacity * c->kv_heads, 4 * (512 / c->head_dim) * RD);
+    const unsigned chunks = row_chunks(c->n_seq, (long)c->capacity * c->kv_heads, 4 * (512 / c->head_dim) * RU);
     SP_REQUIRE(chunks, SPACER_EINVAL, "kv_read: cache too large");
 #define CALL(F, D)                                                                                                                                   \
     do {                                                                                                                                             \

@@ -103,6 +103,29 @@ def test_kv_write_and_read(dev, dtype, n, cap, hkv, d, layout):
     assert same(cut[0], torch.where(keep[..., None, None], got[0].cpu(), torch.zeros(())))
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+@pytest.mark.parametrize("exponent", [-133, -126, -100, -97, -96, -30, 0, 90, 127])
+def test_kv_write_every_quotient(dev, dtype, exponent):
+    """Every bf16 number of the 9 binades below a row's maximum, for every significand of that maximum: codes and scales are exact."""
+    top = torch.arange(128, 256, dtype=F64) * 2.0 ** (exponent - 7)
+    rows = []
+    for shift in range(9):
+        for part in (0, 1):
+            sig = torch.arange(128 + 64 * part, 192 + 64 * part, dtype=F64)
+            x = torch.stack([sig, -sig], 1).view(-1) * 2.0 ** (exponent - 7 - shift)
+            row = x[None].expand(128, -1).clone()
+            row[row.abs() > top[:, None]] = 0.0
+            row[:, 5] = top * (-1) ** shift
+            rows.append(row)
+    x = torch.cat(rows).to(BF)                            # (numbers below 2^-133 round to 0 or to it)
+    n = x.shape[0]
+    cache = make_cache(1, n, 1, 128, dtype, dev)
+    K.kv_write(cache, x.to(dev), x.flip(1).to(dev), torch.arange(n, dtype=torch.int32, device=dev))
+    for codes, scale, want in ((cache.k, cache.k_scale, x), (cache.v, cache.v_scale, x.flip(1))):
+        q, s = codes_ref(want, dtype)
+        assert same(scale[0, 0], s) and same(codes[0, 0].float(), q)
+
+
 @pytest.mark.parametrize("dtype", [BF, E4M3, I8])
 @pytest.mark.parametrize("N,shared", [(1, False), (1, True), (5, False)])
 def test_kv_append(dev, dtype, N, shared):
