@@ -11,8 +11,9 @@
 //                               (lane = column, registers = keys) is the B layout of the second product under a permutation of the keys that the
 //                               image's row order repeats, so no lane exchange lies between the two
 // Work split.  Workgroup = (prompt or sequence, kv head, column block of 16 NC, range of keys); its 4 waves take 32-key tiles in turn and never meet
-// inside the loop: the next tile's K, V and scales are requested before the current one is worked on, so 8 waves per CU keep 64 KB in flight (8 bits).
-// The waves' (O, m, l) are joined through LDS, the ranges' through fp32 records and a second small launch.
+// inside the loop: the next tile's K, V and scales are requested while the current one is worked on, so 8 waves per CU keep 64 KB in flight (8 bits).
+// The waves' (O, m, l) are joined through LDS, the ranges' through fp32 records and a second small launch.  Short contexts take one launch of 8 waves
+// per workgroup that walk the prompt's and the sequence's keys and write the output themselves (plan_attn).
 #include <math.h>
 
 #include "kv_cache.h"
@@ -90,8 +91,8 @@ struct Tile {
 
 // Column blocks of a workgroup: 1 or 2.  (4 leave one lane 128 registers of O: e4m3 rollouts 8 x 8 over 1391 + 300 positions 18.0 instead of 13.8 us, bf16
 // 33 instead of 21; at D = 64 the two are level.)
-constexpr int lds_bytes(int es, int D, int nc) {
-    const int work = 4 * (TK * D * es + 2 * TK * 4), join = nc * 16 * (4 * (D + 4) * 4 + 4 * 8);      // at most 69 KB: two workgroups per CU
+constexpr int lds_bytes(int es, int D, int nc, int nw) {
+    const int work = nw * (TK * D * es + 2 * TK * 4), join = nc * 16 * nw * ((D + 4) * 4 + 8);      // 4 waves: at most 69 KB, two workgroups per CU; 8: 139 KB
     return work > join ? work : join;
 }
 
@@ -104,7 +105,7 @@ struct KeySegment {
 };
 
 // The state of one workgroup's 16 NC columns and what it does with a segment of keys.  ColInfo: (c, row, head, node) -> the query of column c, or false.
-template <int FMT, int D, int NC, class ColInfo>
+template <int FMT, int D, int NC, int NW, class ColInfo>
 struct Columns {
     using T = Tile<FMT, D, NC>;
     static constexpr int DF = D / 16;
@@ -124,7 +125,7 @@ struct Columns {
         : A(args), info(ci), c0(first), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
           g((threadIdx.x & 63) >> 4), scr(0.f), kscr{1.f, 1.f} {
         vimg = smem + wave * T::IMG;
-        sc = (float*)(smem + 4 * T::IMG) + wave * 2 * TK;
+        sc = (float*)(smem + NW * T::IMG) + wave * 2 * TK;
 #pragma unroll
         for (int cb = 0; cb < NC; ++cb) {
             m_run[cb] = -INFINITY; l_run[cb] = 0.f;
@@ -179,12 +180,12 @@ struct Columns {
     }
     __device__ __forceinline__ void fetch(const KeySegment& s, int t) { fetch_k(s, t); fetch_v(s, t); }
 
-    // tiles first, first + 4, ... < s.t1 of a segment; the tile `first` has been requested by fetch()
+    // tiles first, first + NW, ... < s.t1 of a segment; the tile `first` has been requested by fetch()
     __device__ __forceinline__ void run(const KeySegment& s, int first) {
         int t = first;
         const int plain = min(s.t1, s.base / TK);         // from here on some key of a tile is a node or lies behind the last key
-        for (; t < plain; t += 4) tile<false>(s, t);
-        for (; t < s.t1; t += 4) tile<true>(s, t);
+        for (; t < plain; t += NW) tile<false>(s, t);
+        for (; t < s.t1; t += NW) tile<true>(s, t);
     }
 
     template <bool EDGE>
@@ -211,7 +212,7 @@ struct Columns {
                 st[cb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf8[1], qreg[cb][step], st[cb][1], 0, 0, 0);
             }
         }
-        if (t + 4 < s.t1) fetch_k(s, t + 4);              // K's registers are free: the next tile's rows are under way during the rest, V's as soon as
+        if (t + NW < s.t1) fetch_k(s, t + NW);              // K's registers are free: the next tile's rows are under way during the rest, V's as soon as
                                                           // they lie in LDS
         // ---- V and the scales into the wave's image; (the previous tile's LDS reads stay in front of these writes: LDS is in order)
         asm volatile("" ::: "memory");
@@ -227,7 +228,7 @@ struct Columns {
                 for (int e = 0; e < 4; ++e) odd_v |= amax2(w[e]) >= 0x7f80u;
             }
         }
-        if (t + 4 < s.t1) fetch_v(s, t + 4);
+        if (t + NW < s.t1) fetch_v(s, t + NW);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // image and scales complete before any lane reads them
         __builtin_amdgcn_wave_barrier();
         f32x4 ksv[2], vsv[2];
@@ -341,10 +342,10 @@ struct Columns {
 
     // joins the waves ([wave][column][D + 4 floats], [wave][column] (m, l) in LDS) and writes the record `slot` of every column, or with slot < 0 its output
     __device__ __forceinline__ void finish(char* smem, int slot) {
-        constexpr int JC = NC * 16, TPC = 256 / JC, PER = D / TPC;      // columns, threads per column, floats per thread
+        constexpr int JC = NC * 16, TPC = 64 * NW / JC < D / 4 ? 64 * NW / JC : D / 4, PER = D / TPC;      // columns, threads per column, floats per thread
         const int tid = threadIdx.x;
         float* jo = (float*)smem;
-        float2* jm = (float2*)(smem + 4 * JC * (D + 4) * 4);
+        float2* jm = (float2*)(smem + NW * JC * (D + 4) * 4);
         const int jc = tid / TPC, jd = (tid % TPC) * 4;       // (a thread's float4 lie TPC * 4 floats apart: neighbouring threads, neighbouring banks)
         const long ncol_all = (long)A.B * A.N * A.Hq;
         __syncthreads();
@@ -360,12 +361,12 @@ struct Columns {
         }
         __syncthreads();
         int row, head, node;
-        if (!info(c0 + jc, row, head, node)) return;
-        float M = -INFINITY, L = 0.f, f[4];
+        if (jc >= JC || !info(c0 + jc, row, head, node)) return;
+        float M = -INFINITY, L = 0.f, f[NW];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[w * JC + jc].x);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, jm[w * JC + jc].x);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float2 ml = jm[w * JC + jc];
             f[w] = ml.x == -INFINITY ? 0.f : ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
             L += ml.y * f[w];
@@ -377,7 +378,7 @@ struct Columns {
             const int d = jd + i * TPC * 4;
             f32x4 O = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) O += *(const f32x4*)(jo + (w * JC + jc) * (D + 4) + d) * f[w];
+            for (int w = 0; w < NW; ++w) O += *(const f32x4*)(jo + (w * JC + jc) * (D + 4) + d) * f[w];
             if (slot < 0) *(uint2*)(A.o + col * D + d) = make_uint2(pack_bf2(O[0] * inv, O[1] * inv), pack_bf2(O[2] * inv, O[3] * inv));
             else *(f32x4*)(A.rec_o + ((long)slot * ncol_all + col) * D + d) = O;
         }
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
             row = r0 + r; node = A.rep(x); head = hk * rep + x - node * rep;
             return c < ncol;
         };
-        Columns<FMT, D, NCA, decltype(info)> W(A, info, smem, c0);
+        Columns<FMT, D, NCA, 4, decltype(info)> W(A, info, smem, c0);
         if (s.t0 >= s.t1) return W.finish_empty(sp);
         const int first = s.t0 + W.wave;
         if (first < s.t1) W.fetch(s, first);
@@ -450,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
             row = b; node = A.rep(c); head = hk * rep + c - node * rep;
             return c < ncol;
         };
-        Columns<FMT, D, NCB, decltype(info)> W(A, info, smem, c0);
+        Columns<FMT, D, NCB, 4, decltype(info)> W(A, info, smem, c0);
         if (s.t0 >= s.t1) return W.finish_empty(A.sa + sp);
         const int first = s.t0 + W.wave;
         if (first < s.t1) W.fetch(s, first);
@@ -474,7 +475,7 @@ __device__ __forceinline__ int prompt_of_row(const AttnCacheArgs& A, int b) {
 
 // Short contexts: one workgroup takes the prompt's and the sequence's keys of its columns and writes their output itself.
 template <int FMT, int D, int NC>
-__global__ __launch_bounds__(256, 2) void attn_cache_solo_kernel(const AttnCacheArgs A) {
+__global__ __launch_bounds__(512, 2) void attn_cache_solo_kernel(const AttnCacheArgs A) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int rep = A.rep.d, cb = blockIdx.x % A.cbb, hk = (blockIdx.x / A.cbb) % A.Hkv, b = blockIdx.x / (A.cbb * A.Hkv);
     const int ncol = A.N * rep;
@@ -482,7 +483,7 @@ __global__ __launch_bounds__(256, 2) void attn_cache_solo_kernel(const AttnCache
         row = b; node = A.rep(c); head = hk * rep + c - node * rep;
         return c < ncol;
     };
-    Columns<FMT, D, NC, decltype(info)> W(A, info, smem, cb * 16 * NC);
+    Columns<FMT, D, NC, 8, decltype(info)> W(A, info, smem, cb * 16 * NC);
     W.load_queries();
     int nt = 0;
     if (A.n_prompts) {
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void attn_cache_solo_kernel(const AttnCache
     if (A.tail.k) {
         const int base = min(max(A.tail_len[(long)b * A.len_stride], 0), A.tail.cap), total = min(base + A.N, A.tail.cap);
         const KeySegment s = segment_of<FMT>(A.tail, b, hk, total, base, 1, 0);
-        const int first = (W.wave - nt) & 3;              // the waves go on in turn
+        const int first = (W.wave - nt) & 7;              // the waves go on in turn
         if (first < s.t1) W.fetch(s, first);
         W.run(s, first);
     }
@@ -556,8 +557,13 @@ struct AttnPlan {
 
 // How a launch is cut, from the shapes alone (the capacities stand for the lengths, which only the device knows; half of the tail's, which fills up while a
 // rollout runs).
-// Short contexts go in one launch: 640 positions, or 1024 where that launch has 128 workgroups or more (one launch | two: 6.3 | 7.6 us at 384
-// positions of 1 x 2 rollouts, 9.5 | 8.7 at 1024; 8 x 8 rollouts 11.1 | 13.4 us at 1024, 15.3 | 14.5 at 1536).
+// Short contexts go in one launch, whose 8 waves per workgroup walk all keys of its columns and which fills the card once 256 of them (one per CU) are
+// there.  Its bound counts 128-byte key rows per workgroup; both sides measured, one launch | two, e4m3, D = 128 unless said otherwise:
+//   up to 64 workgroups    7.8 |  8.5 us at 700 positions,   9.4 |  8.5 at 1000 (1 x 2 and 1 x 8 rollouts; bf16 crosses at 400)
+//   up to 192             10.0 | 11.5 us at 1013,           13.3 | 12.9 at 1513 (1 x 4 trees of 15)
+//   up to 384             14.2 | 16.1 us at 1903 (8 x 8 rollouts), 21.3 | 23.4 at 3064 (trees of 64), D = 64 16.5 | 17.6 at 3005
+//   more                  13.4 | 14.1 us at 400, but 10 to 20 % slower from 700 on at 512: a second round of workgroups
+// 16 columns per workgroup while these are no more than the CUs (narrow 256: 14.2 us, with 32 columns 16.8; narrow 384, D = 64: 13.6 | 11.9).
 // Others: of the widths (16 or 32 columns) and numbers of key ranges (sa, sb) the one whose estimate (us) is least: 512 workgroups run at once (two per CU), one
 // costs a constant and its 32-key tiles per wave, a record of a column its bytes.  The constants were fitted to 2700 launches of 90 settings (1 to 8
 // prompts of equal and of falling lengths, 1 to 2048 columns, 300 to 14000 positions, all formats): the choice is 3 % behind the best of them in the mean.
@@ -567,9 +573,10 @@ AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, i
     const long positions = (long)(prompt ? prompt->capacity : 0) + (tail ? tail->capacity : 0), narrow = (long)B * c->kv_heads * cdiv(cb, 16);
     AttnPlan p = {};
     p.cols = (long)B * N * Hq;
-    p.solo = positions <= (narrow >= 128 ? 1024 : 640);
+    const long key_rows = positions * c->head_dim * (c->format == KV_BF16 ? 2 : 1) / 128;
+    p.solo = key_rows <= (narrow <= 64 ? 900 : narrow <= 192 ? 1400 : narrow <= 384 ? 3000 : 600);
     if (p.solo) {
-        p.ncb = cb <= 16 || narrow <= 512 ? 1 : 2;
+        p.ncb = cb <= 16 || narrow <= 256 ? 1 : 2;
         p.cbb = cdiv(cb, 16 * p.ncb);
         return p;
     }
@@ -665,10 +672,10 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
         SP_REQUIRE(n <= 0x7fffffffL, SPACER_EINVAL, "attn_cache: too many workgroups");
 #define LAUNCH(F, DD, NC)                                                                                                                           \
     do {                                                                                                                                            \
-        constexpr int lds = lds_bytes(kv_size<F>(), DD, NC);                                                                                         \
+        constexpr int lds = lds_bytes(kv_size<F>(), DD, NC, 8);                                                                                         \
         static const hipError_t once = hipFuncSetAttribute((const void*)attn_cache_solo_kernel<F, DD, NC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
         (void)once;                                                                                                                                 \
-        hipLaunchKernelGGL((attn_cache_solo_kernel<F, DD, NC>), dim3((unsigned)n), dim3(256), lds, s, A);                                            \
+        hipLaunchKernelGGL((attn_cache_solo_kernel<F, DD, NC>), dim3((unsigned)n), dim3(512), lds, s, A);                                            \
     } while (0)
 #define CALL(F, DD)                                                                                                                                 \
     do {                                                                                                                                            \
@@ -687,7 +694,7 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
     A.na = (int)na;
 #define LAUNCH(F, DD, NA, NB)                                                                                                                       \
     do {                                                                                                                                            \
-        constexpr int lds = lds_bytes(kv_size<F>(), DD, NA > NB ? NA : NB);                                                                          \
+        constexpr int lds = lds_bytes(kv_size<F>(), DD, NA > NB ? NA : NB, 4);                                                                          \
         static const hipError_t once = hipFuncSetAttribute((const void*)attn_cache_kernel<F, DD, NA, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
         (void)once;                                                                                                                                 \
         hipLaunchKernelGGL((attn_cache_kernel<F, DD, NA, NB>), dim3((unsigned)(na + nb)), dim3(256), lds, s, A);                                     \
