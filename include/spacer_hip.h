@@ -481,7 +481,7 @@ int spacer_attn_fwd_pair(const void* q_hi, const void* q_lo, const void* k_hi, c
  *   SPACER_KV_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| / scale <= 448
  *   SPACER_KV_INT8  two's complement codes -127 .. 127; scale = max|x| / 127 in fp32, ties of x / scale to even
  * A row with a NaN or an infinity gets scale NaN and codes 0 (it stands for NaN).  Scales of e4m3 rows that a caller makes by other means
- * must be powers of two as well: spacer_attn_cache takes their exponents.
+ * must be powers of two as well: spacer_attn_cache takes their exponents.  Rows may share memory (an expanded view) in a cache that is only read.
  * ---------------------------------------------------------------------------------------------- */
 enum spacer_kv_format { SPACER_KV_BF16 = 0, SPACER_KV_E4M3 = 1, SPACER_KV_INT8 = 2 };
 typedef struct spacer_kv_cache {
@@ -536,7 +536,7 @@ int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache* prompt, c
 /* Marks ids[b * ld + i], i < n (and i < len[b] with len != NULL) as seen in row b, and counts them with counts != NULL.  Ids outside
  * [0, vocab) are skipped. */
 int spacer_token_history_add(int* seen, int* counts, int B, int vocab, const int64_t* ids, long ld, int n, const int* len, spacer_stream_t stream);
-/* out[b, v] (fp32, row stride ld_out; may be the logits themselves) =
+/* out[b, v] (fp32, row stride ld_out; may be the logits themselves, no other overlap) =
  *     x = logits[b, v];  seen: x > 0 ? x / r : x * r;  x -= frequency * count + presence * (count > 0);  x += bias;  not allowed: -infinity
  * computed in 64 bits where a penalty applies and rounded once.  r / frequency / presence: a number for all rows, or fp32 [B] where the pointer
  * is not NULL.  bias fp32 [B, vocab] with row stride ld_bias (0: one row for all), or NULL.  allowed: int32 [n_masks, ceil(vocab / 32)] bit masks

@@ -221,7 +221,15 @@ struct Columns {
 #pragma unroll
         for (int i = 0; i < T::VL; ++i) {
             const int row = lane / T::CPR + i * (64 / T::CPR);
-            *(uint4*)(vimg + row * T::RB + (((lane % T::CPR) ^ T::swz(row)) * 16)) = vr[i];
+            uint4 x = vr[i];
+            if (FMT == KV_E4M3 && EDGE) {                 // a row with a NaN code (the writers make none) counts as NaN: by its scale, which hidden rows drop
+                auto nan4 = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
+                if (nan4(x.x) | nan4(x.y) | nan4(x.z) | nan4(x.w)) {
+                    x = make_uint4(0, 0, 0, 0);
+                    sc[TK + row] = __uint_as_float(0x7fc00000u);
+                }
+            }
+            *(uint4*)(vimg + row * T::RB + (((lane % T::CPR) ^ T::swz(row)) * 16)) = x;
             if (FMT == KV_BF16 && EDGE) {
                 const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll

@@ -232,6 +232,7 @@ int spacer_check_kv_cache(const spacer_kv_cache* c, const char* who) {
     SP_REQUIRE(c->head_dim == 64 || c->head_dim == 128, SPACER_EINVAL, "%s: head_dim %d unsupported (64, 128)", who, c->head_dim);
     SP_REQUIRE(c->n_seq > 0 && c->capacity > 0 && c->kv_heads > 0, SPACER_EINVAL, "%s: empty cache (%d sequences, %d positions, %d heads)", who,
                c->n_seq, c->capacity, c->kv_heads);
+    SP_REQUIRE(c->capacity <= 1 << 30, SPACER_EINVAL, "%s: %d positions (at most 2^30)", who, c->capacity);
     SP_REQUIRE(c->k && c->v, SPACER_EINVAL, "%s: cache without k or v", who);
     const long size = c->format == KV_BF16 ? 2 : 1;
     SP_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0 && ((c->stride_seq | c->stride_head | c->stride_pos) * size) % 16 == 0, SPACER_EINVAL,
@@ -239,6 +240,28 @@ int spacer_check_kv_cache(const spacer_kv_cache* c, const char* who) {
     SP_REQUIRE(c->stride_pos >= 0 && c->stride_pos * size < (1L << 26) && c->scale_stride_pos >= 0 && c->scale_stride_pos < (1L << 26), SPACER_EINVAL,
                "%s: positions of a cache must be less than 64 MiB (scales: 2^26 floats) apart", who);
     SP_REQUIRE(c->format == KV_BF16 || (c->k_scale && c->v_scale), SPACER_EINVAL, "%s: 8-bit cache without scales", who);
+    return SPACER_OK;
+}
+
+// A cache that is written: no two rows (or scales) at one address, as the sequences of an expanded view would be
+static bool apart(const spacer_kv_cache* c, long s0, long s1, long s2, long extent) {
+    long s[3] = {s0, s1, s2}, n[3] = {c->n_seq, c->kv_heads, c->capacity};
+    for (int i = 0; i < 3; ++i) {                         // dimensions by stride, each at least as wide as all below it
+        int at = -1;
+        for (int j = 0; j < 3; ++j)
+            if (n[j] > 1 && (at < 0 || s[j] < s[at])) at = j;
+        if (at < 0) break;
+        if (s[at] < extent) return false;
+        extent += s[at] * (n[at] - 1);
+        n[at] = 1;
+    }
+    return true;
+}
+static int check_target(const spacer_kv_cache* c, const char* who) {
+    if (int rc = spacer_check_kv_cache(c, who)) return rc;
+    SP_REQUIRE(c->k != c->v && apart(c, c->stride_seq, c->stride_head, c->stride_pos, c->head_dim), SPACER_EINVAL, "%s: rows of the cache share memory", who);
+    SP_REQUIRE(c->format == KV_BF16 || (c->k_scale != c->v_scale && apart(c, c->scale_stride_seq, c->scale_stride_head, c->scale_stride_pos, 1)),
+               SPACER_EINVAL, "%s: scales of the cache share memory", who);
     return SPACER_OK;
 }
 
@@ -258,7 +281,7 @@ static int check_source(const void* k, const void* v, long ld, const char* who) 
 }
 
 extern "C" int spacer_kv_write(const spacer_kv_cache* c, const void* k, const void* v, long ld, int n_src, const int* rows, spacer_stream_t stream) {
-    if (int rc = spacer_check_kv_cache(c, "kv_write")) return rc;
+    if (int rc = check_target(c, "kv_write")) return rc;
     SP_REQUIRE(n_src >= 0 && rows, SPACER_EINVAL, "kv_write: rows required, n_src >= 0");
     if (n_src == 0) return SPACER_OK;
     if (int rc = check_source(k, v, ld, "kv_write")) return rc;
@@ -276,7 +299,7 @@ extern "C" int spacer_kv_write(const spacer_kv_cache* c, const void* k, const vo
 
 extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const void* v, long ld, int N, const int* len, int len_per_seq,
                                 spacer_stream_t stream) {
-    if (int rc = spacer_check_kv_cache(c, "kv_append")) return rc;
+    if (int rc = check_target(c, "kv_append")) return rc;
     SP_REQUIRE(N >= 0 && len, SPACER_EINVAL, "kv_append: lengths required, N >= 0");
     if (N == 0) return SPACER_OK;
     if (int rc = check_source(k, v, ld, "kv_append")) return rc;
@@ -315,7 +338,7 @@ extern "C" int spacer_kv_read(const spacer_kv_cache* c, const int* len, void* k_
 extern "C" int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, const float* cos_t, const float* sin_t, void* q_out,
                                               const spacer_kv_cache* c, const int* tail_len, int len_per_seq, const float* rowss, float* rowss_zero,
                                               int norm_cols, float eps, int Hq, spacer_stream_t stream) {
-    if (int rc = spacer_check_kv_cache(c, "decode_qkv_finish_cache")) return rc;
+    if (int rc = check_target(c, "decode_qkv_finish_cache")) return rc;
     const int B = c->n_seq, heads = Hq + 2 * c->kv_heads;
     SP_REQUIRE(acc32 && cos_t && sin_t && q_out && tail_len, SPACER_EINVAL, "decode_qkv_finish_cache: missing operand");
     SP_REQUIRE(Hq > 0, SPACER_EINVAL, "decode_qkv_finish_cache: Hq = %d", Hq);

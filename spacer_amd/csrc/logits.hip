@@ -21,6 +21,7 @@ struct LogitArgs {
 };
 
 constexpr int LU = 4;              // float4 groups per thread
+constexpr int MAX_VOCAB = 1 << 30; // (columns and ids of a row are counted in 32 bits)
 
 template <bool VEC, bool IN_PLACE>
 __global__ __launch_bounds__(256) void process_logits_kernel(const LogitArgs A) {
@@ -166,7 +167,8 @@ __global__ __launch_bounds__(1024) void token_history_row_kernel(int* __restrict
 }  // namespace
 
 extern "C" int spacer_token_history_add(int* seen, int* counts, int B, int vocab, const int64_t* ids, long ld, int n, const int* len, spacer_stream_t stream) {
-    SP_REQUIRE(vocab > 0 && B >= 0 && n >= 0, SPACER_EINVAL, "token_history_add: B = %d, vocab = %d, n = %d", B, vocab, n);
+    SP_REQUIRE(vocab > 0 && vocab <= MAX_VOCAB && B >= 0 && n >= 0 && n <= MAX_VOCAB, SPACER_EINVAL, "token_history_add: B = %d, vocab = %d, n = %d (both at most %d)",
+               B, vocab, n, MAX_VOCAB);
     if (B == 0 || n == 0) return SPACER_OK;
     SP_REQUIRE(seen && ids, SPACER_EINVAL, "token_history_add: seen and ids required");
     SP_REQUIRE(B <= 65535, SPACER_EINVAL, "token_history_add: %d rows (at most 65535)", B);
@@ -182,15 +184,20 @@ extern "C" int spacer_process_logits(const float* logits, long ld, float* out, l
                                      float repetition, const float* repetition_dev, float frequency, const float* frequency_dev, float presence,
                                      const float* presence_dev, const float* bias, long ld_bias, const int* allowed, int n_masks,
                                      const int* allowed_row, spacer_stream_t stream) {
-    SP_REQUIRE(vocab > 0 && B >= 0, SPACER_EINVAL, "process_logits: B = %d, vocab = %d", B, vocab);
+    SP_REQUIRE(vocab > 0 && vocab <= MAX_VOCAB && B >= 0, SPACER_EINVAL, "process_logits: B = %d, vocab = %d (at most %d)", B, vocab, MAX_VOCAB);
     if (B == 0) return SPACER_OK;
     SP_REQUIRE(logits && out, SPACER_EINVAL, "process_logits: logits and out required");
     SP_REQUIRE(B <= 65535, SPACER_EINVAL, "process_logits: %d rows (at most 65535)", B);
+    SP_REQUIRE(B == 1 || (ld >= 0 && ld_out >= vocab), SPACER_EINVAL, "process_logits: rows of out (stride %ld) overlap", ld_out);
+    const bool in_place = logits == out && (ld == ld_out || B == 1);
+    if (!in_place && logits < out + (B - 1) * ld_out + vocab && out < logits + (B - 1) * ld + vocab) {      // side by side in rows of one stride, or refused
+        const long off = ((out - logits) % (ld ? ld : 1) + ld) % (ld ? ld : 1);
+        SP_REQUIRE(B > 1 && ld == ld_out && off >= vocab && off <= ld - vocab, SPACER_EINVAL, "process_logits: out overlaps the logits without being them");
+    }
     SP_REQUIRE(repetition_dev || repetition > 0.f, SPACER_EINVAL, "process_logits: repetition penalty %g must be above 0", (double)repetition);
     SP_REQUIRE(seen || !counts, SPACER_EINVAL, "process_logits: counts without seen");
     SP_REQUIRE(counts || !(frequency_dev || presence_dev || frequency != 0.f || presence != 0.f), SPACER_EINVAL, "process_logits: frequency and presence penalties need counts");
     SP_REQUIRE(!allowed || (allowed_row ? n_masks > 0 : (n_masks == 1 || n_masks == B)), SPACER_EINVAL, "process_logits: %d masks for %d rows", n_masks, B);
-    const bool in_place = logits == out && ld == ld_out;
     LogitArgs A = {logits, out, ld, ld_out, ld_bias, vocab, (vocab + 31) / 32, seen, counts, allowed, allowed_row, n_masks, repetition, frequency, presence,
                    repetition_dev, frequency_dev, presence_dev, bias};
     const bool vec = (((uintptr_t)logits | (uintptr_t)out | (uintptr_t)bias) & 15) == 0 && ((ld | ld_out | (bias ? ld_bias : 0)) & 3) == 0;

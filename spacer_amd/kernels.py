@@ -491,7 +491,8 @@ class KVCache:
     [n_seq, kv_heads, capacity], and stand for code * scale:
         float8_e4m3fn   scale = the smallest power of two >= 2^-126 with max|row| / scale <= 448
         int8            scale = max|row| / 127, codes -127 .. 127, ties of x / scale to even
-    A row that holds a NaN or an infinity gets scale NaN.  (e4m3 scales made elsewhere must be powers of two too.)  The object only describes the tensors (and keeps them alive)."""
+    A row that holds a NaN or an infinity gets scale NaN.  (e4m3 scales made elsewhere must be powers of two too.)  The object only describes the
+    tensors (and keeps them alive); expanded views can be read, not written."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "kv_heads", "capacity", "head_dim", "dtype", "device", "_c", "_ref", "_shape")
 
@@ -515,7 +516,7 @@ class KVCache:
                      and tuple(k_scale.shape) == tuple(v_scale.shape) == (n, h, cap) and k_scale.stride() == v_scale.stride()
                      and k_scale.device == v_scale.device == k.device,
                      "KVCache: an 8-bit cache needs fp32 scales [n_seq, kv_heads, capacity] for k and v, alike in strides")
-            sstride = list(k_scale.stride())
+            sstride = [k_scale.stride(i) if k.shape[i] > 1 else 0 for i in range(3)]
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_seq, self.kv_heads, self.capacity, self.head_dim, self.dtype, self.device = n, h, cap, d, k.dtype, k.device
         self._c = _lib.KvCache(format=_KV_FORMATS[k.dtype], n_seq=n, capacity=cap, kv_heads=h, head_dim=d, k=k.data_ptr(), v=v.data_ptr(),
@@ -540,6 +541,7 @@ class KVCache:
 def _kv_source(cache: KVCache, k, v, what: str) -> int:
     """Number of rows of the source; k and v are alike."""
     rows, cols = k.shape if k.dim() == 2 else (0, 0)
+    _require(rows < 1 << 31, f"{what}: {rows} rows")                                       # (C int)
     if (k.dtype != BF16 or v.dtype != BF16 or cols != cache.kv_heads * cache.head_dim or v.shape != k.shape or v.stride() != k.stride()
             or (rows and k.stride(1) != 1)):
         raise SpacerError(f"{what}: k and v must be bf16 [tokens, kv_heads * head_dim] row-major views with the same strides")
@@ -666,6 +668,7 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
         if n:
             workspace = torch.empty(n, device=q.device, dtype=torch.uint8)
     else:
+        _require(workspace.is_contiguous(), "attn_cache: workspace must be contiguous")
         n = workspace.numel() * workspace.element_size()
     check(_lib.load().spacer_attn_cache(q.data_ptr(), q.stride(0), pr, plen, r0, rows_per_prompt, tl, tlen, per, _addr(tree), tree_per, out.data_ptr(), B, nodes, Hq,
                                         scale, _addr(workspace), n, stream), "attn_cache")
@@ -693,6 +696,7 @@ def token_history_add_(seen, counts, ids, lengths=None, *, vocab: Optional[int] 
     if ids.dtype != torch.int64 or ids.dim() != 2 or (ids.shape[1] > 1 and ids.stride(1) != 1):
         raise SpacerError(f"token_history_add_: ids must be int64 [B, n] with contiguous rows, got {tuple(ids.shape)} {ids.dtype}")
     B, n = ids.shape
+    _require(n <= 1 << 30, f"token_history_add_: {n} ids per row (at most 2^30)")        # (C int)
     vocab = vocab if vocab is not None else counts.shape[1] if counts is not None else seen.shape[1] * 32
     _history(seen, counts, B, vocab, "token_history_add_")
     if lengths is not None:
@@ -725,6 +729,7 @@ def process_logits(logits32, *, seen=None, counts=None, repetition=None, frequen
     if logits32.dtype != torch.float32 or logits32.dim() != 2 or logits32.stride(1) != 1:
         raise SpacerError("process_logits: logits must be fp32 [B, vocab] with contiguous rows")
     B, vocab = logits32.shape
+    _require(vocab <= 1 << 30, f"process_logits: vocabulary of {vocab} (at most 2^30)")       # (C int)
     if out is None:
         out = logits32
     elif out.dtype != torch.float32 or out.shape != logits32.shape or out.stride(1) != 1:

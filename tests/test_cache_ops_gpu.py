@@ -284,6 +284,46 @@ def test_attn_cache(dev, dtype, shape):
         close(got, *attn_ref(q, pval, plens, owner, tval, tlens, masks, hq, d ** -0.5, nodes), what=f"{shape} {dtype}")
 
 
+# every form of the launch (one or two of them, 16 or 32 columns per workgroup for the prompt's and for the sequence's keys) in every format and width
+FORMS = [
+    (4, 4, [100, 1, 0, 77], 40, 5, 64, 16), (1, 3, [1900], 40, 1, 8, 2), (2, 16, [1900, 33], 40, 1, 28, 2), (2, 2, [1, 1900], 40, 21, 8, 2),
+]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, E4M3, I8])
+@pytest.mark.parametrize("form", FORMS)
+def test_attn_cache_forms(dev, dtype, form, d):
+    nP, rows, plens, tcap, nodes, hq, hkv = form
+    B = nP * rows
+    prompt, pval = filled(nP, max(plens), hkv, d, dtype, dev, 61)
+    tail, tval = filled(B, tcap, hkv, d, dtype, dev, 71, "token")
+    tlens = [(13 * b) % (tcap + 1) for b in range(B)]
+    q = (rnd((B * nodes, hq * d), 81) * 1.5).to(BF).to(dev)
+    trees = [random_tree(nodes, 200 + b) for b in range(B)]
+    got = K.attn_cache(q, prompt, torch.tensor(plens, dtype=torch.int32, device=dev), tail, torch.tensor(tlens, dtype=torch.int32, device=dev), hq, d ** -0.5,
+                       rows_per_prompt=rows, nodes=nodes, tree=as_int64(trees, dev))
+    close(got, *attn_ref(q, pval, plens, [b // rows for b in range(B)], tval, tlens, trees, hq, d ** -0.5, nodes), what=f"{form} {dtype} {d}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attn_cache_nan_codes(dev, d):
+    """e4m3 NaN codes (a caller's own: the writers make none) in a drafted node's value row reach the nodes that see it, and no other."""
+    hq, hkv, nodes, B = 4, 2, 5, 2
+    tail, tval = filled(B, 60, hkv, d, E4M3, dev, 2)
+    tlen = [27, 40]
+    for b in range(B):
+        tail.v.view(torch.uint8)[b, :, tlen[b] + 2, d // 2] = 0x7F if b else 0xFF
+        tail.k.view(torch.uint8)[b, :, tlen[b] + 2, 3] = 0x7F
+    q = rnd((B * nodes, hq * d), 3).to(BF).to(dev)
+    masks = [[1, 3, 5, 9, 17], [1, 2, 4, 14, 24]]        # nodes 2 (both) and 3 (second sequence) see node 2
+    got = K.attn_cache(q, None, None, tail, torch.tensor(tlen, dtype=torch.int32, device=dev), hq, 0.1, nodes=nodes, tree=as_int64(masks, dev))
+    sees = torch.tensor([[m >> 2 & 1 for m in row] for row in masks]).bool().view(-1)
+    want, tol = attn_ref(q, None, None, None, tval, tlen, [[m & ~4 for m in row] for row in masks], hq, 0.1, nodes)
+    close(got[~sees.to(dev)], want[~sees], tol[~sees])
+    assert bool(got[sees.to(dev)].isnan().all())
+
+
 @pytest.mark.parametrize("dtype", [BF, I8])
 def test_attn_cache_parts(dev, dtype):
     """Only a prompt, only a tail, ragged prompt owners with sequences that none owns, one length for all, lengths outside the cache."""
@@ -363,12 +403,13 @@ def test_attn_cache_far_offsets_and_spikes(dev):
     close(got, *attn_ref(q, None, None, None, val, [cap - 1], [[1]], hq, d ** -0.5, 1))
 
 
-def test_cache_step_in_graphs(dev):
+@pytest.mark.parametrize("longest", [150, 1900])         # one launch, and two with a workspace
+def test_cache_step_in_graphs(dev, longest):
     """append -> attention captured twice (two graphs, own caches), replayed with lengths and inputs that change on the device, with eager work between the
     replays and on a side stream: every replay equals the eager result bit for bit."""
     hq, hkv, d, B, cap = 14, 2, 128, 6, 90
-    prompt, _ = filled(2, 150, hkv, d, E4M3, dev, 1)
-    pl = torch.tensor([150, 77], dtype=torch.int32, device=dev)
+    prompt, _ = filled(2, longest, hkv, d, E4M3, dev, 1)
+    pl = torch.tensor([longest, 77], dtype=torch.int32, device=dev)
     runs = []
     for i in range(2):
         tail, _ = filled(B, cap, hkv, d, E4M3, dev, 50 + i)

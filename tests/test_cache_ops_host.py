@@ -98,6 +98,39 @@ def test_entries_refuse(lib):
     assert lib.spacer_token_history_add(p, None, 2, 100, p, 4, 0, None, None) == 0
 
 
+def test_written_caches_own_their_rows(lib):
+    """Rows or scales at one address: read, never written.  (With n = 0 a writer that refuses nothing returns before any launch.)"""
+    token_major = dict(stride_seq=64 * 2 * 128, stride_head=128, stride_pos=2 * 128, scale_stride_seq=128, scale_stride_head=1, scale_stride_pos=2)
+    one = dict(n_seq=1, stride_seq=0, scale_stride_seq=0)
+    for good in (dict(), token_major, one, dict(format=_lib.SPACER_KV_BF16, k_scale=None, v_scale=None)):
+        c = cache(**good)
+        assert lib.spacer_kv_write(C.byref(c), 0x10000, 0x10000, 256, 0, 0x10000, None) == 0
+        assert lib.spacer_kv_append(C.byref(c), 0x10000, 0x10000, 256, 0, 0x10000, 0, None) == 0
+    for bad in (dict(stride_seq=0), dict(stride_head=0), dict(stride_pos=0), dict(stride_pos=112), dict(stride_head=63 * 128), dict(v=0x1000), dict(scale_stride_seq=0),
+                dict(scale_stride_head=63), dict(scale_stride_pos=0), dict(v_scale=0x3000), dict(capacity=(1 << 30) + 1)):
+        c, p = cache(**bad), 0x10000
+        assert lib.spacer_kv_write(C.byref(c), p, p, 256, 0, p, None) == EINVAL, bad
+        assert lib.spacer_kv_append(C.byref(c), p, p, 256, 0, p, 0, None) == EINVAL, bad
+        assert lib.spacer_decode_qkv_finish_cache(p, None, p, p, p, C.byref(c), p, 0, None, None, 0, 0.0, 4, None) == EINVAL, bad
+
+
+def test_logits_refuse_overlaps_and_sizes(lib):
+    def logits(x, ld, out, ld_out, B, V=100):
+        # (the history pointers are refused last: an otherwise good call ends at `counts` without `seen`, before any launch)
+        rc = lib.spacer_process_logits(x, ld, out, ld_out, B, V, None, 0x9000, 1.0, None, 0.0, None, 0.0, None, None, 0, None, 0, None, None)
+        assert rc == EINVAL
+        return lib.spacer_last_error().decode()
+    p = 0x100000
+    for good in ((p, 100, p, 100, 4), (p, 104, p, 200, 1), (p, 200, p + 400, 200, 4), (p + 400, 200, p, 200, 4), (p, 0, p + 400, 100, 4), (p, 100, p + 1600, 128, 4)):
+        assert "counts without seen" in logits(*good), good
+    for bad in ((p, 100, p + 4, 100, 4), (p, 100, p, 104, 4), (p, 200, p + 400, 208, 4), (p, 200, p + 396, 200, 4), (p, 200, p + 404, 200, 4), (p, 0, p, 0, 4), (p, 100, p + 4000, 99, 4),
+                (p + 4, 100, p, 100, 1)):
+        assert "overlap" in logits(*bad), bad
+    assert "vocab" in logits(p, 1 << 31, p, 1 << 31, 1, V=(1 << 30) + 1)
+    assert lib.spacer_token_history_add(p, None, 1, (1 << 30) + 1, p, 4, 4, None, None) == EINVAL
+    assert lib.spacer_token_history_add(p, None, 1, 100, p, 1 << 30, (1 << 30) + 1, None, None) == EINVAL
+
+
 def test_python_layer_refuses():
     z = torch.zeros(1, 2, 16, 128, dtype=torch.int8)
     s = torch.zeros(1, 2, 16)
