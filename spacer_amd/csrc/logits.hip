@@ -126,38 +126,57 @@ __global__ __launch_bounds__(256) void process_logits_kernel(const LogitArgs A) 
     }
 }
 
-// Few ids: one thread each.  (A workgroup of the form below would clear and flush a whole bit map for them.)
+// Counts an id per active lane.  Prompts repeat a placeholder token for thousands of positions, and atomics on one address go one by one: lanes that hold
+// the same id as the first one share an atomic, then those of the first one left, the others go alone.  (8 rows of 2051
+// ids, 7/8 of them the same: 37 us without this, 4.4 with it.)
+__device__ __forceinline__ void add_ids(int* counts, int* seen, int v) {
+#pragma unroll
+    for (int round = 0; round < 3; ++round) {
+        const int lead = __builtin_amdgcn_readfirstlane(v);
+        const uint64_t same = round < 2 ? __ballot(v == lead) : 0ull;
+        if (round < 2 && v != lead) continue;
+        if (round == 2 || __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0)) == 0) {
+            if (seen) atomicOr(seen + (v >> 5), (int)(1u << (v & 31)));
+            if (counts) atomicAdd(counts + v, round < 2 ? (int)__popcll(same) : 1);
+        }
+        return;
+    }
+}
+
+// Few ids: one thread each, bits and counts by atomics in memory.
 __global__ __launch_bounds__(256) void token_history_kernel(int* __restrict__ seen, int* __restrict__ counts, int vocab, int words,
                                                             const int64_t* __restrict__ ids, long ld, int n, const int* __restrict__ len) {
     const int b = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
     if (i >= n || (len && i >= len[b])) return;
     const int64_t v = ids[(long)b * ld + i];
     if (v < 0 || v >= vocab) return;
-    atomicOr(seen + (long)b * words + (v >> 5), (int)(1u << (v & 31)));
-    if (counts) atomicAdd(counts + (long)b * vocab + v, 1);
+    add_ids(counts ? counts + (long)b * vocab : nullptr, seen + (long)b * words, (int)v);
 }
 
-// Many ids: one workgroup per row collects the bits in LDS (a prompt repeats its placeholder token thousands of times, and a set bit costs an LDS
-// atomic there instead of one in memory) and owns the row's words, so that they are merged without atomics.
+// Many ids: workgroup 0 of a row collects its bits in LDS and owns the row's words, so that they are merged without atomics; the others count 4096 ids each.
 __global__ __launch_bounds__(1024) void token_history_row_kernel(int* __restrict__ seen, int* __restrict__ counts, int vocab, int words,
                                                                  const int64_t* __restrict__ ids, long ld, int n, const int* __restrict__ len) {
     extern __shared__ int bits[];
-    const int b = blockIdx.x;
+    const int b = blockIdx.y, part = (int)blockIdx.x - 1;
     const int m = len ? min(n, len[b]) : n;
-    for (int i = threadIdx.x; i < words; i += 1024) bits[i] = 0;
-    __syncthreads();
-    for (int i0 = threadIdx.x; i0 < m; i0 += 4 * 1024) {
+    if (part < 0) {
+        for (int i = threadIdx.x; i < words; i += 1024) bits[i] = 0;
+        __syncthreads();
+    }
+    const int end = part < 0 ? m : min(m, (part + 1) * 4096);
+    for (int i0 = max(part, 0) * 4096 + threadIdx.x; i0 < end; i0 += 4096) {
         int64_t v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = i0 + u * 1024 < m ? ids[(long)b * ld + i0 + u * 1024] : -1;
+        for (int u = 0; u < 4; ++u) v[u] = i0 + u * 1024 < end ? ids[(long)b * ld + i0 + u * 1024] : -1;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             if (v[u] < 0 || v[u] >= vocab) continue;
             const int bit = (int)(1u << (v[u] & 31));
-            if (!(bits[v[u] >> 5] & bit)) atomicOr(bits + (v[u] >> 5), bit);
-            if (counts) __hip_atomic_fetch_add(counts + (long)b * vocab + v[u], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (part >= 0) add_ids(counts + (long)b * vocab, nullptr, (int)v[u]);
+            else if (!(bits[v[u] >> 5] & bit)) atomicOr(bits + (v[u] >> 5), bit);
         }
     }
+    if (part >= 0) return;
     __syncthreads();
     int* w = seen + (long)b * words;
     for (int i = threadIdx.x; i < words; i += 1024)
@@ -173,8 +192,11 @@ extern "C" int spacer_token_history_add(int* seen, int* counts, int B, int vocab
     SP_REQUIRE(seen && ids, SPACER_EINVAL, "token_history_add: seen and ids required");
     SP_REQUIRE(B <= 65535, SPACER_EINVAL, "token_history_add: %d rows (at most 65535)", B);
     const int words = (vocab + 31) / 32;
-    if (n >= 256 && words * 4 <= 64 * 1024)      // (256 ids against 4752 words of a 152064-token vocabulary: both forms take the same 6 us at 8 rows)
-        hipLaunchKernelGGL(token_history_row_kernel, dim3(B), dim3(1024), words * 4, (hipStream_t)stream, seen, counts, vocab, words, ids, ld, n, len);
+    // Both forms, few-id | many-id (us, a clear of the bits included, vocabulary 152064): 8 x 2051 ids 4.9 | 7.1, 64 x 1024 8.3 | 6.7, 128 x 1024 13.3 | 9.7,
+    // 128 x 2051 23.0 | 14.7 (different ids, counted: scattered atomics at 28 per ns bound both); with 7/8 of a row the same 4.4 | 6.3, 4.5 | 6.2, 5.2 | 6.7, 7.2 | 7.4
+    if ((long)B * n >= 100000 && words * 4 <= 64 * 1024)
+        hipLaunchKernelGGL(token_history_row_kernel, dim3(1 + (counts ? cdiv(n, 4096) : 0), B), dim3(1024), words * 4, (hipStream_t)stream, seen, counts, vocab, words,
+                           ids, ld, n, len);
     else hipLaunchKernelGGL(token_history_kernel, dim3(cdiv(n, 256), B), dim3(256), 0, (hipStream_t)stream, seen, counts, vocab, words, ids, ld, n, len);
     SP_CHECK_LAUNCH();
     return SPACER_OK;

@@ -525,6 +525,28 @@ def test_process_logits(dev, vocab, B):
             assert inp is view and same(view, got) and bool((wide[:, vocab:] == 99.0).all())
 
 
+@pytest.mark.parametrize("B,n,vocab", [(1, 1, 1), (2, 300, 70), (3, 40000, 1000), (130, 1030, 33), (1, 100001, 152064), (1, 100001, 600000)])
+@pytest.mark.parametrize("kind", ["any", "one", "two"])
+def test_token_history(dev, B, n, vocab, kind):
+    """Runs of one id, ids that alternate, ids outside the vocabulary, rows of every length, a second call on top; rows that share the ids."""
+    g = torch.Generator().manual_seed(n + vocab)
+    ids = torch.randint(-2, vocab + 2, (B, n), generator=g)
+    if kind != "any":
+        ids[:, n // 8:] = torch.tensor([vocab // 2, vocab // 2 if kind == "one" else vocab - 1]).repeat(n)[:n - n // 8]
+    lens = torch.tensor([n, 0, n + 7, n // 2, -1]).repeat(B)[:B].int()
+    seen, counts = K.token_history(B, vocab, dev)
+    K.token_history_add_(seen, counts, ids.to(dev), lens.to(dev))
+    want = torch.stack([torch.bincount(r[:max(int(m), 0)].clamp(-1, vocab) + 1, minlength=vocab + 2)[1:-1] for r, m in zip(ids, lens)])
+    assert torch.equal(counts.cpu().long(), want) and torch.equal(unpack(seen, vocab), want > 0)
+    marked = seen.clone()
+    K.token_history_add_(marked, None, ids[0].to(dev).expand(B, -1), vocab=vocab)
+    first = torch.bincount(ids[0].clamp(-1, vocab) + 1, minlength=vocab + 2)[1:-1]
+    assert torch.equal(unpack(marked, vocab), (want + first) > 0) and torch.equal(counts.cpu().long(), want)
+    K.token_history_add_(seen, counts, ids.to(dev))
+    want = want + torch.stack([torch.bincount(r.clamp(-1, vocab) + 1, minlength=vocab + 2)[1:-1] for r in ids])
+    assert torch.equal(counts.cpu().long(), want) and torch.equal(unpack(seen, vocab), want > 0)
+
+
 def test_sampler_draws_what_the_mask_allows(dev):
     """history -> logits -> sampler, as a decode step runs them: greedy picks the best allowed token that the penalties leave."""
     B, vocab = 4, 2048
