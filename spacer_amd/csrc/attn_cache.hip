@@ -573,8 +573,9 @@ struct AttnPlan {
 //   more                  13.4 | 14.1 us at 400, but 10 to 20 % slower from 700 on at 512: a second round of workgroups
 // 16 columns per workgroup while these are no more than the CUs (narrow 256: 14.2 us, with 32 columns 16.8; narrow 384, D = 64: 13.6 | 11.9).
 // Others: of the widths (16 or 32 columns) and numbers of key ranges (sa, sb) the one whose estimate (us) is least: 512 workgroups run at once (two per CU), one
-// costs a constant and its 32-key tiles per wave, a record of a column its bytes.  The constants were fitted to 2700 launches of 90 settings (1 to 8
-// prompts of equal and of falling lengths, 1 to 2048 columns, 300 to 14000 positions, all formats): the choice is 3 % behind the best of them in the mean.
+// costs a constant and its 32-key tiles per wave, a record of a column its bytes.  The constants were fitted to 2400 launches of 96 settings (1 to 16
+// prompts of equal and of falling lengths, 4 to 4096 columns, 1300 to 30000 positions, all formats): the choice is 3.5 % behind the best of them in the mean.
+// (8 waves per workgroup here too: level with 4 for single long prompts, 2 to 20 % behind elsewhere, so this form has 4.)
 AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
     const spacer_kv_cache* c = prompt ? prompt : tail;
     const long rep = Hq / c->kv_heads, cb = N * rep, ca = prompt ? rows * cb : 0, most = ca > cb ? ca : cb;
@@ -588,22 +589,22 @@ AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, i
         p.cbb = cdiv(cb, 16 * p.ncb);
         return p;
     }
-    static const int ranges[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
-    const double once = 5.9, ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
+    static const int ranges[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+    const double once = 6.7, tile = c->head_dim == 64 ? 0.8 : 1, ta = prompt ? prompt->capacity / (4.0 * TK) : 0, tb = tail ? tail->capacity / (8.0 * TK) : 0;      // tiles per wave
     double best = 1e300;
     for (int nc = 1; nc <= (most > 16 ? 2 : 1); ++nc) {
         const int ncb = cb <= 16 ? 1 : nc, cba = prompt ? cdiv(ca, 16 * nc) : 0, cbb = tail ? cdiv(cb, 16 * ncb) : 0;
         const double ja = (prompt ? (double)prompt->n_seq : 0) * c->kv_heads * cba, jb = (double)B * c->kv_heads * cbb;
-        for (int ia = 0; ia < 13; ++ia) {
+        for (int ia = 0; ia < 10; ++ia) {
             const int sa = prompt ? ranges[ia] : 0;
             if (ia > 0 && (!prompt || ta < sa)) break;
             for (int sb = tail ? 1 : 0; sb <= (tail ? 4 : 0); sb = sb ? 2 * sb : 1) {
                 if (sb > 1 && tb < sb) break;
-                const double a = sa ? ceil(ta / sa) * (0.25 + 0.35 * nc) : 0, b = sb ? ceil(tb / sb) * (0.25 + 0.35 * ncb) : 0;
+                const double a = sa ? ceil(ta / sa) * (0.17 + 0.42 * nc) * tile : 0, b = sb ? ceil(tb / sb) * (0.17 + 0.42 * ncb) * tile : 0;
                 const double work = (ja * sa * (once + a) + jb * sb * (once + b)) / 512, longest = a > b ? a : b;
                 double t = work > longest ? work : longest;
-                if (ja * sa + jb * sb > 512) t += 0.17 * (once + (sa && sb ? (a < b ? a : b) : a + b));
-                t += 0.57e-4 * p.cols * (sa + sb) + 0.53 * cdiv(sa + sb, 8);
+                if (ja * sa + jb * sb > 512) t += 0.19 * (once + (sa && sb ? (a < b ? a : b) : a + b));
+                t += 0.59e-4 * p.cols * (sa + sb) + 0.55 * cdiv(sa + sb, 8);
                 if (t < best) { best = t; p.nca = nc; p.ncb = ncb; p.cba = cba; p.cbb = cbb; p.sa = sa; p.sb = sb; }
             }
         }
