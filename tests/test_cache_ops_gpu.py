@@ -287,6 +287,7 @@ def test_attn_cache(dev, dtype, shape):
 # every form of the launch (one or two of them, 16 or 32 columns per workgroup for the prompt's and for the sequence's keys) in every format and width
 FORMS = [
     (4, 4, [100, 1, 0, 77], 40, 5, 64, 16), (1, 3, [1900], 40, 1, 8, 2), (2, 16, [1900, 33], 40, 1, 28, 2), (2, 2, [1, 1900], 40, 21, 8, 2),
+    (2, 32, [250, 1900], 40, 1, 28, 2), (4, 2, [0, 1900, 65, 320], 70, 64, 16, 2),
 ]
 
 
