@@ -5,7 +5,9 @@
 // Columns and rows.  A column is one query (node i of sequence b, head h); the columns of a kv head that read the same keys are the N side of
 // 16x16x32 bf16 matrix products: the prompt's keys meet every (rollout, node, head) column of the prompt at once, a sequence's own keys its
 // (node, head) columns.  The codes become bf16 in registers (e4m3 and int8 numbers are exact in bf16); s^k multiplies the fp32 scores and s^v
-// the fp32 weights before they are rounded to bf16 for the second product, so no scale costs an operation per element.
+// the fp32 weights before they are rounded to bf16 for the second product, so no scale costs an operation per element.  l sums the weights as rounded, so
+// that a rounding common to numerator and denominator drops out (relative error against 64 bits of 2 x 12 heads over 220 positions, int8: 2.9e-3 with the
+// unrounded sum, now 2.1e-3; the output's own rounding alone gives 1.9e-3).
 //   S^T[key, col] = K . Q^T     A = K rows straight from memory, B = Q fragments
 //   O^T[d, col]  += V^T . P^T   A = V through a wave-private LDS image and the transposing LDS read, B = the weights just computed: the C layout of S^T
 //                               (lane = column, registers = keys) is the B layout of the second product under a permutation of the keys that the
@@ -22,6 +24,7 @@ namespace {
 
 constexpr int TK = 32;            // keys per wave and step
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float TINY = 8.0779357e-28f;      // 2^-90
 
 // n / d for 0 <= n < 2^31 by a multiplication (d is the same for a whole launch): m = floor(2^(31 + s) / d) + 1 with 2^s >= d is exact there
 struct FastDiv {
@@ -91,8 +94,9 @@ struct Tile {
 
 // Column blocks of a workgroup: 1 or 2.  (4 leave one lane 128 registers of O: e4m3 rollouts 8 x 8 over 1391 + 300 positions 18.0 instead of 13.8 us, bf16
 // 33 instead of 21; at D = 64 the two are level.)
+constexpr int SCALES = TK * (4 + 4 + 2 + 2);      // a wave's row scales: K's (int8), V's, and 1 / V's as two bf16 numbers
 constexpr int lds_bytes(int es, int D, int nc, int nw) {
-    const int work = nw * (TK * D * es + 2 * TK * 4), join = nc * 16 * nw * ((D + 4) * 4 + 8);      // 4 waves: at most 69 KB, two workgroups per CU; 8: 139 KB
+    const int work = nw * (TK * D * es + SCALES), join = nc * 16 * nw * ((D + 4) * 4 + 8);      // 4 waves: at most 69 KB, two workgroups per CU; 8: 139 KB
     return work > join ? work : join;
 }
 
@@ -125,7 +129,7 @@ struct Columns {
         : A(args), info(ci), c0(first), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
           g((threadIdx.x & 63) >> 4), scr(0.f), kscr{1.f, 1.f} {
         vimg = smem + wave * T::IMG;
-        sc = (float*)(smem + NW * T::IMG) + wave * 2 * TK;
+        sc = (float*)(smem + NW * T::IMG + wave * SCALES);
 #pragma unroll
         for (int cb = 0; cb < NC; ++cb) {
             m_run[cb] = -INFINITY; l_run[cb] = 0.f;
@@ -216,7 +220,18 @@ struct Columns {
                                                           // they lie in LDS
         // ---- V and the scales into the wave's image; (the previous tile's LDS reads stay in front of these writes: LDS is in order)
         asm volatile("" ::: "memory");
-        if (FMT != KV_BF16) sc[lane] = FMT == KV_INT8 && lane < TK ? scr * (A.scale * LOG2E) : scr;
+        uint16_t* inv_v = (uint16_t*)(sc + 2 * TK);       // [2][TK]
+        bool tiny = false;                                // a V row below 2^-90 (a row of zeros): its weights are counted before they meet the scale
+        if (FMT != KV_BF16) {
+            sc[lane] = FMT == KV_INT8 && lane < TK ? scr * (A.scale * LOG2E) : scr;
+            if (lane >= TK) {
+                const float inv = scr >= TINY && scr < INFINITY ? __builtin_amdgcn_rcpf(scr) : 0.f;
+                const uint32_t hi = pack_bf2(inv, 0.f) & 0xffffu;
+                inv_v[lane - TK] = (uint16_t)hi;
+                if (FMT == KV_INT8) inv_v[lane] = (uint16_t)pack_bf2(inv - __uint_as_float(hi << 16), 0.f);
+            }
+            tiny = __any(lane >= TK && scr < TINY);
+        }
         bool odd_v = false;                               // a NaN or an infinity in a bf16 V row that some columns must not see
 #pragma unroll
         for (int i = 0; i < T::VL; ++i) {
@@ -287,20 +302,43 @@ struct Columns {
                 for (int d = 0; d < DF; ++d) oacc[cb][d] *= alpha;
             }
             const float m = EDGE && m_run[cb] == -INFINITY ? 0.f : m_run[cb];     // nothing seen yet: every weight is 0
-            float sum = 0.f;
 #pragma unroll
             for (int kf = 0; kf < 2; ++kf)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[kf][r] = __builtin_amdgcn_exp2f(FMT == KV_INT8 ? p[kf][r] - m : fmaf(p[kf][r], kmul, -m));
-                    sum += p[kf][r];
-                    if (FMT != KV_BF16) {
+                for (int r = 0; r < 4; ++r) p[kf][r] = __builtin_amdgcn_exp2f(FMT == KV_INT8 ? p[kf][r] - m : fmaf(p[kf][r], kmul, -m));
+            if (FMT != KV_BF16) {
+                if (tiny) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sum += vsv[kf][r] < TINY ? p[kf][r] : 0.f;
+                    sum += __shfl_xor(sum, 16, 64);
+                    l_run[cb] += sum + __shfl_xor(sum, 32, 64);
+                }
+#pragma unroll
+                for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
                         p[kf][r] *= vsv[kf][r];
                         if (EDGE && !vis[kf][r]) p[kf][r] = 0.f;    // (the scale of a hidden row may be NaN)
                     }
+            }
+            const uint4 pk = make_uint4(pack_bf2(p[0][0], p[0][1]), pack_bf2(p[0][2], p[0][3]), pack_bf2(p[1][0], p[1][1]), pack_bf2(p[1][2], p[1][3]));
+            pf[cb] = __builtin_bit_cast(bf16x8, pk);
+            // the sum counts the weights as the second product sees them, rounded: a row's rounding then scales numerator and denominator alike, and
+            // a key that outweighs the others comes out exactly
+            if (FMT == KV_BF16) {
+                l_run[cb] += ((bf_lo(pk.x) + bf_hi(pk.x)) + (bf_lo(pk.y) + bf_hi(pk.y))) + ((bf_lo(pk.z) + bf_hi(pk.z)) + (bf_lo(pk.w) + bf_hi(pk.w)));
+            } else {                                      // ... without the scale they carry: one more product, with 1 / s^v (e4m3: exact; int8: to 2^-17)
+                f32x4 sum = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int part = 0; part < (FMT == KV_INT8 ? 2 : 1); ++part) {
+                    const uint2 a = *(const uint2*)(inv_v + part * TK + 4 * g), b = *(const uint2*)(inv_v + part * TK + 16 + 4 * g);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y)), pf[cb], sum, 0, 0, 0);
                 }
-            l_run[cb] += sum;
-            pf[cb] = __builtin_bit_cast(bf16x8, make_uint4(pack_bf2(p[0][0], p[0][1]), pack_bf2(p[0][2], p[0][3]), pack_bf2(p[1][0], p[1][1]), pack_bf2(p[1][2], p[1][3])));
+                l_run[cb] += sum[0];
+            }
         }
         // ---- O^T += V^T . P^T; slot j of lane group g is key (j >> 2) * 16 + 4 g + (j & 3)
         if (FMT == KV_BF16 && EDGE && __any(odd_v)) {     // rare: a product with a hidden NaN or infinity would be NaN; add visible keys one by one
@@ -360,8 +398,10 @@ struct Columns {
 #pragma unroll
         for (int r = 0; r < NC; ++r) {
             float l = l_run[r];
-            l += __shfl_xor(l, 16, 64);
-            l += __shfl_xor(l, 32, 64);
+            if (FMT == KV_BF16) {                         // (8-bit: every lane of a column holds its sum)
+                l += __shfl_xor(l, 16, 64);
+                l += __shfl_xor(l, 32, 64);
+            }
 #pragma unroll
             for (int df = 0; df < DF; ++df)
                 *(f32x4*)(jo + (wave * JC + r * 16 + l15) * (D + 4) + df * 16 + g * 4) = oacc[r][df];

@@ -2,7 +2,9 @@
 
 Codes, scales, bit maps and counts are compared exactly.  Attention: with A = sum_j w_j |v_j| of an output (w the softmax weights) an error is at most
   2^-8 |o|            the output's own rounding to bf16
-  2^-8 A              every weight is rounded to bf16 for the second product (the sum of the weights is not)
+  2^-8 M + 2^-13 A    every weight is rounded to bf16 by a factor 1 + d_j, |d_j| <= 2^-8, and the sum counts the rounded ones: the quotient is off by
+                      sum_j w_j d_j (v_j - o) / (1 + sum_j w_j d_j), with M = sum_j w_j |v_j - o| <= 2 A at most 2^-8 M (1 + 2^-7); int8 sums are off by
+                      another 2^-17 (a reciprocal in two bf16 numbers): 2^-15 M + 2^-17 |o| <= 2^-13 A in all beside 2^-8 M
   2 E A               E bounds the scores' error in 32 bits: (D + 4) 2^-24 max_j sum_d |q_d k_jd| scale (products and sums), + 2^-21 for exp2 and its argument
 """
 import math
@@ -221,7 +223,8 @@ def attn_ref(q, prompt, plen, owner, tail, tlen, masks, hq, scale, nodes):
             w = torch.softmax(x, -1)
             o, a = torch.einsum("hl,hld->hd", w, v), torch.einsum("hl,hld->hd", w, v.abs())
             e = (d + 4) * 2.0 ** -24 * torch.einsum("hd,hld->hl", q[b, i].abs(), k.abs()).amax(-1) * scale + 2.0 ** -21
-            out[b, i], tol[b, i] = o, 2.0 ** -8 * (o.abs() + a) + 2 * e[:, None] * a
+            spread = torch.einsum("hl,hld->hd", w, (v - o[:, None]).abs())
+            out[b, i], tol[b, i] = o, 2.0 ** -8 * (o.abs() + spread) + 2.0 ** -13 * a + 2 * e[:, None] * a
     return out.view(B * nodes, hq * d), tol.view(B * nodes, hq * d)
 
 
@@ -357,6 +360,23 @@ def test_attn_cache_rows_that_see_nothing(dev, dtype):
     close(got, want, tol)
     for row in (0, 2, 3, 4):
         assert float(got[row].float().abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [BF, E4M3, I8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("every", [2, 3, 70])            # of so many rows one is ordinary (70: the first of them), the others zero or of 2^-100
+def test_attn_cache_rows_of_zeros(dev, dtype, d, every):
+    """Rows of zeros and rows far below the others carry weight and add nothing."""
+    hq, hkv, B, cap, nodes = 8, 2, 2, 69, 3
+    tail = make_cache(B, cap, hkv, d, dtype, dev)
+    size = torch.tensor([1.0 if i % every == 0 else 0.0 if i % 2 else 2.0 ** -100 for i in range(B * cap)], dtype=F64)
+    k, v = rnd((B * cap, hkv * d), 5).to(BF), (rnd((B * cap, hkv * d), 6) * size[:, None]).to(BF)
+    K.kv_write(tail, k.to(dev), v.to(dev), torch.arange(B * cap, dtype=torch.int32, device=dev))
+    val = [x.double().cpu().transpose(1, 2) for x in K.kv_read(tail, dtype=F32)]
+    q = rnd((B * nodes, hq * d), 7).to(BF).to(dev)
+    tlen, masks = [66, 35], [chain(nodes)] * B
+    got = K.attn_cache(q, None, None, tail, torch.tensor(tlen, dtype=torch.int32, device=dev), hq, d ** -0.5, nodes=nodes)
+    close(got, *attn_ref(q, None, None, None, val, tlen, masks, hq, d ** -0.5, nodes))
 
 
 @pytest.mark.parametrize("dtype", [BF, E4M3, I8])
