@@ -16,6 +16,10 @@
 // inside the loop: the next tile's K, V and scales are requested while the current one is worked on, so 8 waves per CU keep 64 KB in flight (8 bits).
 // The waves' (O, m, l) are joined through LDS, the ranges' through fp32 records and a second small launch.  Short contexts take one launch of 8 waves
 // per workgroup that walk the prompt's and the sequence's keys and write the output themselves (plan_attn).
+// Measured (kernels alone): 2 x 12 heads over 220 int8 positions 6.2 us; 8 x 8 rollouts x 28 heads over 1391 + 300 e4m3 positions 14 us, over 16384 + 700 of
+// int8 42 + 5 (join); 8 trees of 13 over 2311 + 211 bf16 positions 16 + 4; 32 trees of 32 over 5498 + 333 e4m3 positions of D = 64 50 + 5.  Many columns per
+// key are bound by the softmax's and the conversions' VALU work (about 160 operations and 16 exponentials beside 18 products a tile of 32 x 32, D = 64), few by
+// the latency of a tile's rows.
 #include <math.h>
 
 #include "kv_cache.h"

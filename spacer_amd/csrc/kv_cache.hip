@@ -5,7 +5,9 @@
 //   kv_read     the cache's values as bf16 or fp32 rows [sequence, position, kv head, D]
 //   decode_qkv_finish_cache   the decode step's form of kv_append: split-K sums + bias + rotary -> q, and K / V into the cache
 //
-// All four move each byte once and are bound by memory: D / 8 lanes hold a row (16-byte loads), K and V of a row are in flight together.
+// All four move each byte once and are bound by memory: D / 8 lanes hold a row (16-byte loads), K and V of a row are in flight together.  Measured, D = 128:
+// 4 prompts of up to 16384 positions x 4 heads to e4m3 39.6 us (181 MB, 4.6 TB/s) and back to bf16 35.7 us (203 MB, 5.7 TB/s); 8 x 1391 x 4 to int8 10.0 us
+// and back to fp32 13.5 us; a step's 64 tokens x 4 heads 3.8 us, which is a launch.
 #include "kv_cache.h"
 
 namespace {
@@ -45,6 +47,7 @@ __device__ __forceinline__ void store_row(char* dst, float* scale, const uint4 x
 // Rows of a pass: sequence (blockIdx.x / chunks, a scalar), then row = position * Hkv + head inside it (32 bits), so that the heads of a token,
 // side by side in the source, fall to one wave.  A lane holds a piece of RU rows of K and V: all loads are in flight before the first use, without a
 // branch between them (rows that are not stored read row 0).
+// (1 row a lane 40 us for the 16384-position prompts, 4 rows or several steps per workgroup 58.)
 constexpr int RU = 2;
 template <int D> constexpr int rows_per_block() { return 4 * (512 / D) * RU; }
 
