@@ -13,6 +13,10 @@ namespace {
 constexpr int SNT = 1024;
 constexpr int CAP = 1024;    // candidate capacity (top_k <= CAP; ties beyond CAP are dropped)
 
+// The least key of a logit above -infinity.  Forbidden tokens are no candidates: where fewer than top_k tokens are allowed they would be ties of the
+// top_k-th largest logit, and more of them than CAP would push allowed tokens out of the list.
+constexpr uint32_t KEY_FINITE = 0x00800000u;
+
 __device__ __forceinline__ uint32_t okey(float x) {
     const uint32_t u = __float_as_uint(x);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
     // values) that is then trimmed exactly after the sort.  Pathological rows (mass ties) overflow CAP and take the
     // exact 4-pass radix select over the whole row.
     bool trimmed_exactly = false;
-    const bool pre = pre_n && pre_n[b] <= CAP;
+    const bool pre = pre_n && pre_n[b] <= CAP && pre_n[b] > 0;
     if (pre) {
         if (tid == 0) ncand = pre_n[b];
         if (tid < pre_n[b]) { cval[tid] = pre_val[(long)b * CAP + tid]; cidx[tid] = pre_idx[(long)b * CAP + tid]; }
@@ -177,10 +181,12 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
     __syncthreads();
     const uint32_t bound = kth_key([&](int i) { return cval[i]; }, SNT, top_k);
     __syncthreads();
-    gather(bound);
+    gather(max(bound, KEY_FINITE));
+    const bool none = ncand == 0;                         // every token forbidden: some token, as there is no answer
+    if (none) gather(bound);
     if (ncand > CAP) {
         const uint32_t kth = kth_key(val, vocab, top_k);
-        gather(kth);
+        gather(none ? kth : max(kth, KEY_FINITE));
         trimmed_exactly = true;
     }
     }
@@ -304,7 +310,7 @@ __global__ __launch_bounds__(SNT) void sample_gather_kernel(const float* __restr
     for (int i = tid; i < S * SNT; i += SNT) mx[i] = pmax[(long)b * S * SNT + i];
     if (tid == 0) nloc = 0;
     __syncthreads();
-    const uint32_t thr = kth_key_fn([&](int i) { return mx[i]; }, S * SNT, top_k, hist, sel_bin, sel_k);
+    const uint32_t thr = max(kth_key_fn([&](int i) { return mx[i]; }, S * SNT, top_k, hist, sel_bin, sel_k), KEY_FINITE);
     const float* row = logits + (long)b * ld;
     auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
     auto consider = [&](float x, int i) {

@@ -584,3 +584,36 @@ def test_sampler_draws_what_the_mask_allows(dev):
         drawn.append(ids.cpu())
     order = torch.argsort(x.cpu()[:, 100:200], dim=1, descending=True)[:, :5] + 100
     assert torch.equal(torch.stack(drawn, 1), order)
+
+
+@pytest.mark.parametrize("n", [1, 2, 49, 50, 700, 5000])
+@pytest.mark.parametrize("wide", [False, True])
+def test_sampler_with_few_allowed_tokens(dev, n, wide):
+    """A mask that leaves fewer tokens than top_k of a large vocabulary: the draw is the one from these tokens alone (same order, same numbers, same uniform)."""
+    B, vocab = 8, 151936
+    x = rnd((B, vocab), 15).float().to(dev)
+    ids = torch.randperm(vocab, generator=torch.Generator().manual_seed(n))[:n].sort().values
+    allowed = torch.zeros(1, vocab, dtype=torch.bool)
+    allowed[0, ids] = True
+    logits = K.process_logits(x, allowed=pack(allowed).to(dev), out=torch.empty_like(x))
+    alone = x[:, ids.to(dev)].contiguous()
+    ws = K.sample_workspace(B, vocab, dev) if wide else None
+    for step in range(4):
+        at = torch.tensor([step], dtype=torch.int32, device=dev)
+        for top_k, top_p in ((1, 1.0), (50, 0.9), (50, 1.0)):
+            got = K.sample_top_p(logits, at, top_k=top_k, top_p=top_p, seed=3, workspace=ws)
+            want = K.sample_top_p(alone, at, top_k=min(top_k, n), top_p=top_p, seed=3)
+            assert torch.equal(ids.to(dev)[want], got), (step, top_k, top_p)
+
+
+def test_sampler_where_nothing_is_allowed(dev):
+    """All of a row forbidden: some token of the vocabulary, beside rows that are not disturbed."""
+    B, vocab = 4, 151936
+    x = rnd((B, vocab), 15).float().to(dev)
+    allowed = torch.ones(B, vocab, dtype=torch.bool)
+    allowed[1] = False
+    logits = K.process_logits(x, allowed=pack(allowed).to(dev), out=torch.empty_like(x))
+    at = torch.zeros(1, dtype=torch.int32, device=dev)
+    for ws in (None, K.sample_workspace(B, vocab, dev)):
+        got, want = K.sample_top_p(logits, at, seed=3, workspace=ws), K.sample_top_p(x, at, seed=3)
+        assert torch.equal(got[[0, 2, 3]], want[[0, 2, 3]]) and 0 <= int(got[1]) < vocab
