@@ -126,10 +126,10 @@ class _LogitRules:
             allowed = torch.zeros(vocab, dtype=torch.bool)
             allowed[ids] = True
         drawable = allowed.clone() if bias is None else allowed & (bias > float("-inf"))
-        if sp.suppress_eos:
+        if sp.suppress_eos or sp.synthetic_lengths:
             drawable[eos_id] = False
         if not bool(drawable.any()):
-            raise ValueError("SamplingParams: allowed_token_ids, logit_bias and suppress_eos leave no token to draw")
+            raise ValueError("SamplingParams: allowed_token_ids, logit_bias and suppress_eos / synthetic_lengths leave no token to draw")
         self.penalties = dict(repetition=float(sp.repetition_penalty), frequency=float(sp.frequency_penalty), presence=float(sp.presence_penalty))
         if not 0.0 < self.penalties["repetition"] < float("inf") or any(not abs(self.penalties[n]) < float("inf") for n in ("frequency", "presence")):
             raise ValueError(f"SamplingParams: penalties {self.penalties}: finite numbers, the repetition penalty above 0")

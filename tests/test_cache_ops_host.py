@@ -154,3 +154,23 @@ def test_python_layer_refuses():
         K.token_history_add_(torch.zeros(2, 1, dtype=torch.int32), None, torch.zeros(2, 4, dtype=torch.int32))
     with pytest.raises(K.SpacerError, match="cache"):
         K.attn_cache(torch.zeros(2, 128, dtype=torch.bfloat16), None, None, None, None, 1, 1.0)
+
+
+def test_logit_rules_refuse_and_pack():
+    """SamplingParams' rules: what leaves nothing to draw or is no number is refused before any kernel; the allowed ids as bits."""
+    from spacer_amd.rollout import SamplingParams, _LogitRules
+    inf, nan = float("inf"), float("nan")
+
+    def rules(**kw):
+        sp = SamplingParams(**kw)
+        assert _LogitRules.wanted(sp)
+        return _LogitRules(sp, [], [1], 100, 7, "cpu")
+    for kw in (dict(logit_bias={100: 1.0}), dict(logit_bias={-1: 1.0}), dict(logit_bias={3: nan}), dict(logit_bias={3: inf}), dict(allowed_token_ids=[]), dict(allowed_token_ids=[100]),
+               dict(allowed_token_ids=[5, -1]), dict(allowed_token_ids=[3], logit_bias={3: -inf}), dict(allowed_token_ids=[7], suppress_eos=True), dict(allowed_token_ids=[7], synthetic_lengths=(2, 4)), dict(repetition_penalty=0.0),
+               dict(repetition_penalty=-1.0), dict(repetition_penalty=nan), dict(repetition_penalty=inf), dict(frequency_penalty=nan), dict(presence_penalty=-inf)):
+        with pytest.raises(ValueError):
+            rules(**kw)
+    assert not _LogitRules.wanted(SamplingParams())
+    r = rules(allowed_token_ids=[0, 31, 32, 99, 99], logit_bias={2: -inf, 99: 0.5})
+    assert r.allowed.tolist() == [[(1 << 31 | 1) - 2 ** 32, 1, 0, 8]] and r.seen is None
+    assert r.bias[2] == -inf and r.bias[99] == 0.5 and int((r.bias != 0).sum()) == 2
