@@ -625,7 +625,7 @@ def attn_cache_workspace_bytes(prompt: Optional[KVCache], tail: Optional[KVCache
     return n
 
 
-def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache], tail_len, Hq, scale, *, rows_per_prompt=1, row0=None, nodes=1,
+def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache], tail_len, Hq, scale, *, rows_per_prompt=None, row0=None, nodes=1,
                tree=None, out=None, workspace=None):
     """Decode attention over caches in any format, for one new token per sequence (``nodes`` = 1) or a tree of up to 64 drafted tokens.
 
@@ -633,8 +633,9 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
     sequence's positions [0, tail_len[b]) in ``tail``, and the nodes j whose bit j is set in its mask, node j being at position tail_len[b] + j of
     ``tail`` (append the nodes first: ``kv_append`` / ``decode_qkv_finish_cache``).  ``tree``: int64 [nodes] (one tree for all sequences) or
     [B, nodes]; None: node i sees the nodes up to and including itself.  A node that sees nothing gets zeros.
-    ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` sequences from
-    p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt each.
+    ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` (None: 1) sequences from
+    p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt (None: B)
+    each -- more is the caller's error and not noticed.
     prompt_len int32 [n_prompts]; tail_len int32 [B] or [1]; scale > 0.  ``workspace``: attn_cache_workspace_bytes bytes; None allocates it."""
     c = prompt if prompt is not None else tail
     if c is None:
@@ -643,6 +644,8 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
     if q.dtype != BF16 or width != Hq * c.head_dim or nodes < 1 or rows_q % nodes or q.stride(1) != 1:
         raise SpacerError(f"attn_cache: q must be bf16 [B * nodes, Hq * head_dim] with contiguous rows, got {tuple(q.shape)} {q.dtype}, {nodes} nodes")
     B = rows_q // nodes
+    if rows_per_prompt is None:
+        rows_per_prompt = 1 if row0 is None else max(B, 1)
     pr = plen = r0 = tl = tlen = None
     per = tree_per = 0
     if prompt is not None:

@@ -349,6 +349,38 @@ def test_attn_cache_parts(dev, dtype):
     close(K.attn_cache(q, None, None, tail, far, hq, s), *attn_ref(q, None, None, None, tval, far.tolist(), masks, hq, s, 1))
 
 
+@pytest.mark.parametrize("longest", [45, 1900])          # one launch, and two
+def test_attn_cache_uneven_owners(dev, longest):
+    """row0 alone: any number of sequences per prompt, none, and sequences of no prompt in front and behind."""
+    hq, hkv, d, B = 7, 1, 128, 9
+    prompt, pval = filled(4, longest, hkv, d, E4M3, dev, 1)
+    tail, tval = filled(B, 33, hkv, d, E4M3, dev, 2)
+    q = rnd((B, hq * d), 3).to(BF).to(dev)
+    plen, tlen, masks = [longest, 7, 33, longest - 1], list(range(B)), [[1]] * B
+    row0 = torch.tensor([1, 6, 6, 7, 8], dtype=torch.int32, device=dev)
+    got = K.attn_cache(q, prompt, torch.tensor(plen, dtype=torch.int32, device=dev), tail, torch.tensor(tlen, dtype=torch.int32, device=dev), hq, d ** -0.5, row0=row0)
+    close(got, *attn_ref(q, pval, plen, [None, 0, 0, 0, 0, 0, 2, 3, None], tval, tlen, masks, hq, d ** -0.5, 1))
+
+
+@pytest.mark.parametrize("dtype", [BF, I8])
+def test_expanded_cache(dev, dtype):
+    """One sequence's rows seen as several: read like copies, refused by the writers."""
+    hq, hkv, d, B = 4, 2, 64, 3
+    one, val = filled(1, 40, hkv, d, dtype, dev, 1)
+    shared = K.KVCache(*(None if x is None else x.expand(B, *x.shape[1:]) for x in (one.k, one.v, one.k_scale, one.v_scale)))
+    k, _ = K.kv_read(shared, dtype=F32)
+    assert torch.equal(k.double().cpu().transpose(1, 2), val[0].expand(B, -1, -1, -1))
+    q = rnd((B, hq * d), 3).to(BF).to(dev)
+    n = [3, 39, 20]
+    got = K.attn_cache(q, None, None, shared, torch.tensor(n, dtype=torch.int32, device=dev), hq, 0.1)
+    close(got, *attn_ref(q, None, None, None, [x.expand(B, -1, -1, -1) for x in val], n, [[1]] * B, hq, 0.1, 1))
+    rows = torch.zeros(B, hkv * d, device=dev, dtype=BF)
+    with pytest.raises(K.SpacerError, match="share memory"):
+        K.kv_append(shared, rows, rows, torch.tensor(n, dtype=torch.int32, device=dev))
+    with pytest.raises(K.SpacerError, match="share memory"):
+        K.kv_write(shared, rows, rows, torch.zeros(B * 40, device=dev, dtype=torch.int32))
+
+
 @pytest.mark.parametrize("dtype", [BF, E4M3, I8])
 def test_attn_cache_rows_that_see_nothing(dev, dtype):
     hq, hkv, d, nodes = 4, 2, 128, 3
