@@ -369,6 +369,8 @@ int spacer_scatter_f32(const float* src, const int64_t* idx, float* dst, long n,
  * Sampling (HF generate with do_sample, temperature 1, top_k, top_p; TR:277-284).  logits fp32 [B, vocab].
  * One token per row into out_ids[b].  finished[b] != 0 rows emit pad_id.  Philox counter = (seed, step, b).
  * suppress_eos != 0 forbids eos_id (fixed-length throughput mode).
+ * Forbidden (-infinite) logits are never drawn while another is left, and a NaN logit counts as one; a row without any other gives some token
+ * of the vocabulary.
  * ---------------------------------------------------------------------------------------------- */
 int spacer_sample_top_p(const float* logits, long ld, int B, int vocab, int top_k, float top_p, float temperature,
                         uint64_t seed, const int* step_dev, int eos_id, int pad_id, int suppress_eos, int* finished,

@@ -17,6 +17,11 @@ constexpr int CAP = 1024;    // candidate capacity (top_k <= CAP; ties beyond CA
 // top_k-th largest logit, and more of them than CAP would push allowed tokens out of the list.
 constexpr uint32_t KEY_FINITE = 0x00800000u;
 
+// A NaN logit is a forbidden one.  No comparison places it: the sort would leave it (or a filler of the sort) anywhere, a top_k-th value of NaN would
+// keep no candidate and a negative NaN lies below -infinity's key, so that no candidate would be found at all -- the token would then be read from
+// in front of the list.  With NaN as -infinity every row has a candidate: what is above -infinity, or (nothing is) all of the row.
+__device__ __forceinline__ float never_nan(float x) { return x == x ? x : -INFINITY; }
+
 __device__ __forceinline__ uint32_t okey(float x) {
     const uint32_t u = __float_as_uint(x);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
@@ -129,7 +134,7 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
         return;
     }
     const float* row = logits + (long)b * ld;
-    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
+    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : never_nan(raw * inv_temp); };
     auto val = [&](int i) -> float { return fix(row[i], i); };
     const bool vec_ok = (ld % 4 == 0) && (((uintptr_t)logits & 15) == 0);
 
@@ -283,7 +288,7 @@ __global__ __launch_bounds__(SNT) void sample_partmax_kernel(const float* __rest
     if (sl == 0 && tid == 0) pre_n[b] = 0;
     if (finished && finished[b]) return;
     const float* row = logits + (long)b * ld;
-    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
+    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : never_nan(raw * inv_temp); };
     const int n4 = vocab >> 2, per = (n4 + S - 1) / S, q0 = sl * per, q1 = min(n4, q0 + per);
     float lmax = -INFINITY;
     for (int i4 = q0 + tid; i4 < q1; i4 += SNT) {
@@ -312,7 +317,7 @@ __global__ __launch_bounds__(SNT) void sample_gather_kernel(const float* __restr
     __syncthreads();
     const uint32_t thr = max(kth_key_fn([&](int i) { return mx[i]; }, S * SNT, top_k, hist, sel_bin, sel_k), KEY_FINITE);
     const float* row = logits + (long)b * ld;
-    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
+    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : never_nan(raw * inv_temp); };
     auto consider = [&](float x, int i) {
         if (okey(x) >= thr) {
             const int slot = atomicAdd(&nloc, 1);
