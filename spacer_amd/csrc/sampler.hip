@@ -240,20 +240,21 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
     // ---- 4. draw
     const int step_now = *step_dev + step_bias;
     const float u = philox_uniform(seed, (uint32_t)step_now, (uint32_t)b) * Zk;
-    __shared__ int chosen;
-    if (tid == 0) chosen = -1;
+    __shared__ int chosen, last;
+    if (tid == 0) chosen = last = -1;
     __syncthreads();
     if (keep && exk <= u && u < exk + pk) chosen = tid;     // at most one thread satisfies this
     __syncthreads();
-    if (chosen < 0) {   // numeric edge (u == Zk after rounding): take the last kept candidate
-        const int cand = keep ? tid : -1;
-        int best = cand;
+    int pick = chosen;
+    if (pick < 0) {   // numeric edge (u == Zk after rounding): take the last kept candidate (in a word of its own: a wave may still be about to read `chosen`)
+        int best = keep ? tid : -1;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
-        if (lane == 0) atomicMax(&chosen, best);
+        if (lane == 0) atomicMax(&last, best);
         __syncthreads();
+        pick = last;
     }
-    const int tok = cidx[chosen];
+    const int tok = cidx[pick];
     if (out_logp) {     // log-prob of the drawn token under the full (untruncated) softmax
         float m = -INFINITY;
         for (int i = tid; i < vocab; i += SNT) m = fmaxf(m, val(i));
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
         float s = 0.f;
         for (int i = tid; i < vocab; i += SNT) s += __expf(val(i) - M);
         const float S = block_sum(s, red);
-        if (tid == 0) out_logp[b] = cval[chosen] - M - logf(S);
+        if (tid == 0) out_logp[b] = cval[pick] - M - logf(S);
     }
     if (tid == 0) {
         out_ids[b] = tok;

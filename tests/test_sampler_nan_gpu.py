@@ -70,3 +70,25 @@ def test_nan_among_logits(dev, vocab, share, negative):
                     out.append((K.sample_top_p(row, at, top_k=top_k, top_p=top_p, seed=3, out_logp=logp, workspace=ws), logp))
                 assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
                 assert not bool(where[torch.arange(B), out[0][0].cpu()].any())
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_edge_of_the_draw_with_log_probabilities(dev, wide):
+    """Rows whose draw no candidate's interval takes (sums that are no numbers: an infinite logit, nothing allowed) beside ordinary ones, with the pass for the
+    log-probability behind them: the infinite logit is drawn, ordinary rows are not disturbed."""
+    B, vocab = 64, 151936
+    x = logits(B, vocab).to(dev)
+    clean = x.clone()
+    x[::4, 777] = math.inf
+    x[1::4] = -math.inf
+    at = torch.zeros(1, dtype=torch.int32, device=dev)
+    ws = K.sample_workspace(B, vocab, dev) if wide else None
+    want_p = torch.zeros(B, device=dev)
+    want = K.sample_top_p(clean, at, seed=3, out_logp=want_p, workspace=ws)
+    for _ in range(4):
+        logp = torch.zeros(B, device=dev)
+        got = K.sample_top_p(x, at, seed=3, out_logp=logp, workspace=ws)
+        for r in (2, 3):
+            assert torch.equal(got[r::4], want[r::4]) and torch.equal(logp[r::4], want_p[r::4])
+        assert bool((got[::4] == 777).all()) and bool(logp[::4].isnan().all()) and bool(logp[1::4].isnan().all())
+        assert bool(((got >= 0) & (got < vocab)).all())
