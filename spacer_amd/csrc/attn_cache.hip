@@ -436,7 +436,7 @@ struct Columns {
         }
         if (slot >= 0 && tid % TPC == 0) A.rec_ml[(long)slot * ncol_all + col] = make_float2(M, L);
     }
-    // no keys: the columns' records say so by their maximum alone
+    // no keys: the columns' records say so by their maximum and their sum, and hold no O
     __device__ __forceinline__ void finish_empty(int slot) const {
         int row, head, node;
         if (threadIdx.x < NC * 16 && info(c0 + threadIdx.x, row, head, node))
@@ -592,7 +592,8 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(const AttnCacheArg
         for (int e = 0; e < 4; ++e) O[e] *= f0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (s0 + i >= ns || ml[i].x == -INFINITY) continue;
+            // an empty range has no O and says so by its sum; NaN scores alone leave the maximum at -infinity too, but a sum of NaN, which stays
+            if (s0 + i >= ns || (ml[i].x == -INFINITY && ml[i].y == 0.f)) continue;
             const float f = ml[i].x == M ? 1.f : __builtin_amdgcn_exp2f(ml[i].x - M);
             L += ml[i].y * f;
             O[0] += x[i].x * f; O[1] += x[i].y * f; O[2] += x[i].z * f; O[3] += x[i].w * f;

@@ -1,0 +1,85 @@
+"""attn_cache where numbers stop being finite and where callers leave the ordinary layouts, in the one-launch form (short capacities) and in the two-launch
+one, whose key ranges meet in a second kernel.  Both have to give the definition's answer: the launch is chosen by capacities, not by the data.
+Reference and tolerances: test_cache_ops_gpu.attn_ref."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from spacer_amd import kernels as K        # noqa: E402
+from test_cache_ops_gpu import BF, E4M3, F32, I8, attn_ref, close, filled, make_cache, rnd  # noqa: E402
+
+FORMATS = [BF, E4M3, I8]
+LONGEST = [45, 1900]                       # prompt capacities: one launch, two launches
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def forms(prompt, tail, rows, B, hq, longest):
+    """The capacities take the form that the case is about."""
+    assert (K.attn_cache_workspace_bytes(prompt, tail, rows, B, 1, hq) > 0) == (longest == LONGEST[1])
+
+
+def poison(cache, which, seq, head, positions):
+    """The rows of one kv head become what the writers make of a row with a NaN: scale NaN and codes 0, in bf16 the row itself with a NaN in it."""
+    for x, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        if (x is cache.k) == (which == "k"):
+            if s is None:
+                x[seq, head, positions, 5] = math.nan
+            else:
+                s[seq, head, positions] = math.nan
+                x.view(torch.uint8)[seq, head, positions] = 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("longest", LONGEST)
+def test_nan_query(dev, dtype, d, longest):
+    """A query head with a NaN gives NaN, wherever its keys lie; the others what they gave."""
+    hq, hkv, B = 12, 2, 4
+    prompt, pval = filled(2, longest, hkv, d, dtype, dev, 1)
+    tail, tval = filled(B, 40, hkv, d, dtype, dev, 2)
+    forms(prompt, tail, 2, B, hq, longest)
+    q = rnd((B, hq, d), 3).to(BF)
+    bad = torch.zeros(B, hq, dtype=torch.bool)
+    for b, h in ((0, 0), (1, 11), (3, 5)):
+        q[b, h, 7 + h] = math.nan
+        bad[b, h] = True
+    plen, tlen = [longest, longest // 2], [0, 3, 39, 17]
+    got = K.attn_cache(q.view(B, -1).to(dev), prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=2).view(B, hq, d)
+    want, tol = attn_ref(torch.where(bad[..., None], 0.0, q).view(B, -1), pval, plen, [0, 0, 1, 1], tval, tlen, [[1]] * B, hq, d ** -0.5, 1)
+    assert bool(got[bad.to(dev)].isnan().all())
+    close(got[~bad.to(dev)], want.view(B, hq, d)[~bad], tol.view(B, hq, d)[~bad])
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("longest", LONGEST)
+@pytest.mark.parametrize("part", ["prompt", "own", "one of the prompt"])
+def test_nan_rows_of_a_whole_range(dev, dtype, which, longest, part):
+    """NaN rows reach every column that sees them, also where they are all that a range of keys holds (a rollout's first own token, a whole prompt)."""
+    hq, hkv, d, B = 8, 2, 128, 4
+    prompt, pval = filled(2, longest, hkv, d, dtype, dev, 1)
+    tail, tval = filled(B, 40, hkv, d, dtype, dev, 2)
+    forms(prompt, tail, 2, B, hq, longest)
+    plen, tlen = [longest, longest - 5], [0, 0, 3, 39]
+    bad = torch.zeros(B, hq, dtype=torch.bool)
+    if part == "own":
+        poison(tail, which, 1, 0, slice(0, 1))
+        bad[1, :4] = True
+    else:
+        poison(prompt, which, 1, 1, slice(0, longest) if part == "prompt" else slice(longest // 2, longest // 2 + 1))
+        bad[2:, 4:] = True
+    q = rnd((B, hq * d), 3).to(BF)
+    got = K.attn_cache(q.to(dev), prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=2).view(B, hq, d)
+    want, tol = attn_ref(q, pval, plen, [0, 0, 1, 1], tval, tlen, [[1]] * B, hq, d ** -0.5, 1)      # (values read before the rows were spoiled)
+    close(got[~bad.to(dev)], want.view(B, hq, d)[~bad], tol.view(B, hq, d)[~bad])
+    hit = got[bad.to(dev)].isnan()
+    if which == "v" and dtype == BF:                      # a NaN number of a value row is one channel's
+        assert bool(hit[:, 5].all()) and not bool(hit[:, :5].any()) and not bool(hit[:, 6:].any())
+    else:
+        assert bool(hit.all())
