@@ -305,7 +305,7 @@ struct Columns {
 #pragma unroll
                 for (int d = 0; d < DF; ++d) oacc[cb][d] *= alpha;
             }
-            const float m = EDGE && m_run[cb] == -INFINITY ? 0.f : m_run[cb];     // nothing seen yet: every weight is 0
+            const float m = m_run[cb] == -INFINITY ? 0.f : m_run[cb];     // nothing seen yet, or only scores of -infinity: every weight is 0
 #pragma unroll
             for (int kf = 0; kf < 2; ++kf)
 #pragma unroll

@@ -632,7 +632,8 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
     q bf16 [B * nodes, Hq * head_dim] (row b * nodes + i = node i of sequence b).  Node i sees its prompt's positions [0, prompt_len[p]), its
     sequence's positions [0, tail_len[b]) in ``tail``, and the nodes j whose bit j is set in its mask, node j being at position tail_len[b] + j of
     ``tail`` (append the nodes first: ``kv_append`` / ``decode_qkv_finish_cache``).  ``tree``: int64 [nodes] (one tree for all sequences) or
-    [B, nodes]; None: node i sees the nodes up to and including itself.  A node that sees nothing gets zeros.
+    [B, nodes]; None: node i sees the nodes up to and including itself.  A node that sees nothing, or only scores of -inf, gets
+    zeros; a NaN that it sees gives NaN.
     ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` (None: 1) sequences from
     p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt (None: B)
     each -- more is the caller's error and not noticed.

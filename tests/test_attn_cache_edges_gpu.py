@@ -83,3 +83,22 @@ def test_nan_rows_of_a_whole_range(dev, dtype, which, longest, part):
         assert bool(hit[:, 5].all()) and not bool(hit[:, :5].any()) and not bool(hit[:, 6:].any())
     else:
         assert bool(hit.all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("longest", LONGEST)
+@pytest.mark.parametrize("first", [0, 64])
+def test_scores_of_minus_infinity(dev, d, longest, first):
+    """Keys whose score is -infinity weigh nothing, also where a wave meets nothing else in its first tiles."""
+    hq, hkv, B, n = 8, 2, 4, 32 if longest == LONGEST[0] else 640
+    prompt, pval = filled(2, longest, hkv, d, BF, dev, 1)
+    tail, tval = filled(B, 40, hkv, d, BF, dev, 2)
+    forms(prompt, tail, 2, B, hq, longest)
+    first = min(first, longest - n)
+    q = rnd((B, hq, d), 3).to(BF)
+    q[..., 9] = q[..., 9].abs() + 0.5
+    prompt.k[:, :, first:first + n, 9] = -math.inf
+    plen, tlen = [longest, longest], [0, 3, 39, 17]
+    keep = [i for i in range(longest) if not first <= i < first + n]
+    want = attn_ref(q.view(B, -1), [x[:, :, keep] for x in pval], [len(keep)] * 2, [0, 0, 1, 1], tval, tlen, [[1]] * B, hq, d ** -0.5, 1)
+    close(K.attn_cache(q.view(B, -1).to(dev), prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=2), *want)
