@@ -186,13 +186,14 @@ __global__ __launch_bounds__(256) void decode_qkv_finish_cache_kernel(float* __r
     const int j = min(lane, half - 1);
     const bool on = lane < half;
     float* a = acc + (long)wid * D;
-    // every load before the first use: absent operands read a valid dummy address and are masked
+    // every load before the first use: absent operands read a valid dummy address, whose bits (those of a float: they may spell an infinity or NaN, which a
+    // product with 0 would keep) are cleared
     const bf16_t* bias_p = bias ? bias + (long)hh * D : (const bf16_t*)cs;
     const float bias_on = bias ? 1.f : 0.f;
     const int pos = tail_len[(long)b * len_stride];
     const float rsum = rowss ? rowss[b] : 0.f;
     const float a1 = a[j], a2 = a[j + half];
-    const bf16_t b1 = bias_p[bias ? j : 0], b2 = bias_p[bias ? j + half : 0];
+    const bf16_t bias_bits = bias ? 0xffffu : 0u, b1 = bias_p[bias ? j : 0] & bias_bits, b2 = bias_p[bias ? j + half : 0] & bias_bits;
     const float c1 = cs[(long)b * D + j], s1 = sn[(long)b * D + j], c2 = cs[(long)b * D + j + half], s2 = sn[(long)b * D + j + half];
     const float rs = rowss ? rsqrtf(rsum / (float)norm_cols + eps) : 1.f;
     float x1 = a1 * rs + bias_on * bf2f(b1), x2 = a2 * rs + bias_on * bf2f(b2);
