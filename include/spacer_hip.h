@@ -519,8 +519,8 @@ int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, const float* 
  *   the positions [0, prompt_len[p]) of its prompt p in `prompt` (shared by the prompt's sequences; NULL: no prompt),
  *   the positions [0, tail_len[b]) of sequence b in `tail` (NULL: none), and
  *   the nodes j whose bit j is set in tree[b * tree_per_seq * N + i] (int64; NULL: j <= i), node j at position tail_len[b] + j of `tail`.
- * Prompt p owns the sequences [row0[p], row0[p + 1]) (int32 [n_prompts + 1] on the device, ascending), or with row0 NULL
- * [p * rows, (p + 1) * rows); at most `rows` of them.  Lengths are clamped to the caches.  A node that sees nothing, or
+ * Prompt p owns the sequences [row0[p], row0[p + 1]) (int32 [n_prompts + 1] on the device, ascending; `rows` = as many as a prompt usually has:
+ * what the launch is cut for, more are served in a second round), or with row0 NULL [p * rows, (p + 1) * rows).  Lengths are clamped to the caches.  A node that sees nothing, or
  * only keys whose score is -infinity, gets zeros; a NaN that it sees (query, key or value row) gives NaN.
  * scale > 0.  o bf16 [B * N, Hq * head_dim] contiguous.  prompt and tail share format, kv_heads and head_dim; tail->n_seq = B.
  * workspace: spacer_attn_cache_workspace_bytes(...) bytes of device memory, 16-byte aligned, no initialisation; the cache structs may be NULL

@@ -129,9 +129,9 @@ struct Columns {
     uint4 kr[2][T::KL], vr[T::VL];
     float scr, kscr[2];               // row scales: of V (lanes 32 .., e4m3: all lanes) and of K (int8: lanes .. 31; e4m3: kscr, a lane's own rows)
 
-    __device__ __forceinline__ Columns(const AttnCacheArgs& args, const ColInfo& ci, char* smem, int first)
-        : A(args), info(ci), c0(first), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
-          g((threadIdx.x & 63) >> 4), scr(0.f), kscr{1.f, 1.f} {
+    __device__ __forceinline__ Columns(const AttnCacheArgs& args, const ColInfo& ci, char* smem, int first, int tid = threadIdx.x)
+        : A(args), info(ci), c0(first), lane(tid & 63), wave(__builtin_amdgcn_readfirstlane(tid >> 6)), l15(tid & 15),
+          g((tid & 63) >> 4), scr(0.f), kscr{1.f, 1.f} {
         vimg = smem + wave * T::IMG;
         sc = (float*)(smem + NW * T::IMG + wave * SCALES);
 #pragma unroll
@@ -460,10 +460,12 @@ __device__ __forceinline__ KeySegment segment_of(const KvView& c, int seq, int h
 __device__ __forceinline__ void rows_of(const AttnCacheArgs& A, int pr, int& r0, int& r1) {
     r0 = A.row0 ? min(max(A.row0[pr], 0), A.B) : min(pr * A.rows, A.B);
     r1 = A.row0 ? min(max(A.row0[pr + 1], r0), A.B) : min((pr + 1) * A.rows, A.B);
-    r1 = min(r1, r0 + A.rows);
 }
 
-template <int FMT, int D, int NCA, int NCB>
+// AGAIN: row0 may give a prompt more sequences than the launch was cut for (A.rows); a workgroup then goes on to the columns behind the launch's.  A form of
+// its own, for row0 with rows below the batch, because the loop costs registers: 80 rollouts of 12 prompts (8 or 4 each) over 1391 and 16384 positions take
+// 26.9 and 122 us with it and 23.0 and 112 without in bf16, 8-bit caches are level (e4m3 27.2 and 55.3, int8 31.5 and 70.8).
+template <int FMT, int D, int NCA, int NCB, bool AGAIN>
 __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs A) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int rep = A.rep.d;
@@ -476,7 +478,8 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
         if (pr >= A.n_prompts) return;
         int r0, r1;
         rows_of(A, pr, r0, r1);
-        const int per_row = A.N * rep, ncol = (r1 - r0) * per_row, c0 = cb * 16 * NCA;
+        const int per_row = A.N * rep, ncol = (r1 - r0) * per_row;
+        int c0 = cb * 16 * NCA, tid = threadIdx.x;
         if (c0 >= ncol) return;
         const int total = min(max(A.prompt_len[pr], 0), A.prompt.cap);
         const KeySegment s = segment_of<FMT>(A.prompt, pr, hk, total, total, A.sa, sp);
@@ -485,13 +488,20 @@ __global__ __launch_bounds__(256, 2) void attn_cache_kernel(const AttnCacheArgs 
             row = r0 + r; node = A.rep(x); head = hk * rep + x - node * rep;
             return c < ncol;
         };
-        Columns<FMT, D, NCA, 4, decltype(info)> W(A, info, smem, c0);
-        if (s.t0 >= s.t1) return W.finish_empty(sp);
-        const int first = s.t0 + W.wave;
-        if (first < s.t1) W.fetch(s, first);
-        W.load_queries();
-        W.run(s, first);
-        W.finish(smem, sp);
+        do {
+            if (AGAIN) asm volatile("" : "+v"(tid));      // (addresses from the lane's number are worked out anew, not kept from round to round)
+            Columns<FMT, D, NCA, 4, decltype(info)> W(A, info, smem, c0, tid);
+            if (s.t0 >= s.t1) W.finish_empty(sp);
+            else {
+                const int first = s.t0 + W.wave;
+                if (first < s.t1) W.fetch(s, first);
+                W.load_queries();
+                W.run(s, first);
+                W.finish(smem, sp);
+            }
+            c0 += A.cba * 16 * NCA;
+            if (AGAIN) __syncthreads();                   // the join's reads of LDS stay in front of the next columns' writes
+        } while (AGAIN && c0 < ncol);
     } else {
         const int sp = job % A.sb, hk = (job / A.sb) % A.Hkv, b = job / (A.sb * A.Hkv);
         if (b >= A.B) return;
@@ -746,12 +756,18 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
     const long na = (ja + 7) / 8 * 8 * p.cba, nb = (jb + 7) / 8 * 8 * p.cbb;
     SP_REQUIRE(na + nb <= 0x7fffffffL, SPACER_EINVAL, "attn_cache: too many workgroups");
     A.na = (int)na;
-#define LAUNCH(F, DD, NA, NB)                                                                                                                       \
+    const bool again = row0 && rows < B;
+#define LAUNCH_AS(F, DD, NA, NB, AGAIN)                                                                                                             \
     do {                                                                                                                                            \
         constexpr int lds = lds_bytes(kv_size<F>(), DD, NA > NB ? NA : NB, 4);                                                                          \
-        static const hipError_t once = hipFuncSetAttribute((const void*)attn_cache_kernel<F, DD, NA, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
+        static const hipError_t once = hipFuncSetAttribute((const void*)attn_cache_kernel<F, DD, NA, NB, AGAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
         (void)once;                                                                                                                                 \
-        hipLaunchKernelGGL((attn_cache_kernel<F, DD, NA, NB>), dim3((unsigned)(na + nb)), dim3(256), lds, s, A);                                     \
+        hipLaunchKernelGGL((attn_cache_kernel<F, DD, NA, NB, AGAIN>), dim3((unsigned)(na + nb)), dim3(256), lds, s, A);                              \
+    } while (0)
+#define LAUNCH(F, DD, NA, NB)                                                                                                                       \
+    do {                                                                                                                                            \
+        if (again) LAUNCH_AS(F, DD, NA, NB, true);                                                                                                  \
+        else LAUNCH_AS(F, DD, NA, NB, false);                                                                                                       \
     } while (0)
 #define CALL(F, DD)                                                                                                                                 \
     do {                                                                                                                                            \
@@ -762,6 +778,7 @@ extern "C" int spacer_attn_cache(const void* q, long q_ld, const spacer_kv_cache
     KV_DISPATCH(c, CALL);
 #undef CALL
 #undef LAUNCH
+#undef LAUNCH_AS
     if (D == 128) hipLaunchKernelGGL(attn_cache_join_kernel<128>, dim3(cdiv(p.cols, 8)), dim3(256), 0, s, A);
     else hipLaunchKernelGGL(attn_cache_join_kernel<64>, dim3(cdiv(p.cols, 16)), dim3(256), 0, s, A);
     SP_CHECK_LAUNCH();

@@ -635,8 +635,8 @@ def attn_cache(q, prompt: Optional[KVCache], prompt_len, tail: Optional[KVCache]
     [B, nodes]; None: node i sees the nodes up to and including itself.  A node that sees nothing, or only scores of -inf, gets
     zeros; a NaN that it sees gives NaN.
     ``prompt`` None: sequences without a prompt; ``tail`` None: prompts only.  Prompt p serves the ``rows_per_prompt`` (None: 1) sequences from
-    p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]), at most rows_per_prompt (None: B)
-    each -- more is the caller's error and not noticed.
+    p * rows_per_prompt on, or with ``row0`` (int32 [n_prompts + 1], ascending) the sequences [row0[p], row0[p + 1]); rows_per_prompt (None: B) is then what
+    the launch is cut for, and prompts with more are served in a second round.
     prompt_len int32 [n_prompts]; tail_len int32 [B] or [1]; scale > 0.  ``workspace``: attn_cache_workspace_bytes bytes; None allocates it."""
     c = prompt if prompt is not None else tail
     if c is None:

@@ -102,3 +102,22 @@ def test_scores_of_minus_infinity(dev, d, longest, first):
     keep = [i for i in range(longest) if not first <= i < first + n]
     want = attn_ref(q.view(B, -1), [x[:, :, keep] for x in pval], [len(keep)] * 2, [0, 0, 1, 1], tval, tlen, [[1]] * B, hq, d ** -0.5, 1)
     close(K.attn_cache(q.view(B, -1).to(dev), prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=2), *want)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("longest", LONGEST)
+@pytest.mark.parametrize("rows", [1, 2, 5])
+def test_prompts_of_more_sequences_than_rows_per_prompt(dev, dtype, longest, rows):
+    """With row0 the number of sequences per prompt is row0's: rows_per_prompt only says what to launch for."""
+    hq, hkv, d, B, nodes = 14, 2, 128, 14, 2
+    prompt, pval = filled(4, longest, hkv, d, dtype, dev, 1)
+    tail, tval = filled(B, 40, hkv, d, dtype, dev, 2)
+    forms(prompt, tail, rows, B, hq, longest)
+    row0 = [1, 6, 6, 13, 14]
+    owner = [None] + [0] * 5 + [2] * 7 + [3]
+    plen, tlen = [longest, 7, 33, longest - 1], [2 * b for b in range(B)]
+    q = rnd((B * nodes, hq * d), 3).to(BF).to(dev)
+    n = K.attn_cache_workspace_bytes(prompt, tail, rows, B, nodes, hq)
+    ws = torch.full((n,), 0x7F, dtype=torch.uint8, device=dev)              # what nobody wrote is huge
+    got = K.attn_cache(q, prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=rows, row0=i32(row0, dev), nodes=nodes, workspace=ws)
+    close(got, *attn_ref(q, pval, plen, owner, tval, tlen, [[1, 3]] * B, hq, d ** -0.5, nodes))
