@@ -73,6 +73,10 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint2 w, float s) {
     return __builtin_bit_cast(bf16x8, make_uint4(o[0], o[1], o[2], o[3]));
 }
 
+// An e4m3 scale that is neither a power of two of 2^-126 or more nor 0: the conversion above takes its exponent alone, and the sum of the rounded weights
+// its reciprocal as a bf16 number, so that it would be one number here and another to kv_read
+__device__ __forceinline__ bool no_power_of_two(float s) { return (__float_as_uint(s) & 0x807fffffu) != 0u; }
+
 // maximum over the four 16-lane groups (lanes of the same column)
 __device__ __forceinline__ float group_max(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -127,7 +131,7 @@ struct Columns {
     f32x4 oacc[NC][DF];
     float m_run[NC], l_run[NC];
     uint4 kr[2][T::KL], vr[T::VL];
-    float scr, kscr[2];               // row scales: of V (lanes 32 .., e4m3: all lanes) and of K (int8: lanes .. 31; e4m3: kscr, a lane's own rows)
+    float scr, kscr[2];               // row scales: of K (lanes .. 31) and of V (lanes 32 ..); e4m3: kscr, K's again for the rows that a lane converts
 
     __device__ __forceinline__ Columns(const AttnCacheArgs& args, const ColInfo& ci, char* smem, int first, int tid = threadIdx.x)
         : A(args), info(ci), c0(first), lane(tid & 63), wave(__builtin_amdgcn_readfirstlane(tid >> 6)), l15(tid & 15),
@@ -177,7 +181,7 @@ struct Columns {
         const int k0 = t * TK, last = s.total - 1 - k0;
         const char* vb = s.v + (long)k0 * s.row_b;
         if (FMT != KV_BF16) {
-            const float* sb = (FMT == KV_E4M3 || lane >= TK ? s.vs : s.ks) + (long)k0 * s.c_pos;
+            const float* sb = (lane >= TK ? s.vs : s.ks) + (long)k0 * s.c_pos;
             scr = sb[min(lane & (TK - 1), last) * s.c_pos];
         }
 #pragma unroll
@@ -228,6 +232,8 @@ struct Columns {
         bool tiny = false;                                // a V row below 2^-90 (a row of zeros): its weights are counted before they meet the scale
         if (FMT != KV_BF16) {
             sc[lane] = FMT == KV_INT8 && lane < TK ? scr * (A.scale * LOG2E) : scr;
+            // (rare) a key whose K or V scale is no power of two counts as NaN, by its V scale, which hidden keys drop
+            if (FMT == KV_E4M3 && __any(no_power_of_two(scr)) && no_power_of_two(scr)) sc[TK + (lane & (TK - 1))] = __uint_as_float(0x7fc00000u);
             if (lane >= TK) {
                 const float inv = scr >= TINY && scr < INFINITY ? __builtin_amdgcn_rcpf(scr) : 0.f;
                 const uint32_t hi = pack_bf2(inv, 0.f) & 0xffffu;

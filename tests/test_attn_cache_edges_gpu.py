@@ -121,3 +121,46 @@ def test_prompts_of_more_sequences_than_rows_per_prompt(dev, dtype, longest, row
     ws = torch.full((n,), 0x7F, dtype=torch.uint8, device=dev)              # what nobody wrote is huge
     got = K.attn_cache(q, prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=rows, row0=i32(row0, dev), nodes=nodes, workspace=ws)
     close(got, *attn_ref(q, pval, plen, owner, tval, tlen, [[1, 3]] * B, hq, d ** -0.5, nodes))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("scale", [3.0, -2.0, 2.0 ** -130, 0.3])
+@pytest.mark.parametrize("longest", LONGEST)
+def test_e4m3_scales_that_are_no_powers_of_two(dev, d, which, scale, longest):
+    """attn_cache takes e4m3 scales by their exponents: any other number in a row that is seen gives NaN and nobody else is touched; 0 is the scale of a row of zeros."""
+    hq, hkv, B = 8, 2, 4
+    prompt, pval = filled(2, longest, hkv, d, E4M3, dev, 1)
+    tail, tval = filled(B, 40, hkv, d, E4M3, dev, 2)
+    s = dict(k=(prompt.k_scale, tail.k_scale), v=(prompt.v_scale, tail.v_scale))[which]
+    s[0][1, 1, 33] = scale                                # a key of the second prompt, kv head 1
+    s[1][0, 0, 5] = scale                                 # the newest key of the first sequence, kv head 0
+    s[1][1, :, 6:] = scale                                # behind the newest key of the second: nobody's
+    for x, t in ((tail.k, tail.k_scale), (tail.v, tail.v_scale)):
+        x.view(torch.uint8)[2, 0, 1] = 0
+        t[2, 0, 1] = 0.0
+    tval = [x.clone() for x in tval]
+    for x in tval:
+        x[2, 0, 1] = 0.0
+    bad = torch.zeros(B, hq, dtype=torch.bool)
+    bad[2:, 4:] = True
+    bad[0, :4] = True
+    q = rnd((B, hq * d), 3).to(BF)
+    plen, tlen = [longest, longest], [5, 5, 3, 39]
+    got = K.attn_cache(q.to(dev), prompt, i32(plen, dev), tail, i32(tlen, dev), hq, d ** -0.5, rows_per_prompt=2).view(B, hq, d)
+    want, tol = attn_ref(q, pval, plen, [0, 0, 1, 1], tval, tlen, [[1]] * B, hq, d ** -0.5, 1)
+    close(got[~bad.to(dev)], want.view(B, hq, d)[~bad], tol.view(B, hq, d)[~bad])
+    assert bool(got[bad.to(dev)].isnan().all())
+    if which == "k" and scale > 1:                        # a hidden node's own
+        nodes = 3
+        q = rnd((B * nodes, hq * d), 4).to(BF)
+        s[1][:, :, 20] = scale
+        masks = [[1, 1, 5]] * B
+        tree = torch.tensor(masks[0], dtype=torch.int64, device=dev)
+        got = K.attn_cache(q.to(dev), None, None, tail, i32([19] * B, dev), hq, d ** -0.5, nodes=nodes, tree=tree).view(B * nodes, hq, d)
+        want, tol = attn_ref(q, None, None, None, tval, [19] * B, masks, hq, d ** -0.5, nodes)
+        fine = torch.ones(B, nodes, hq, dtype=torch.bool)
+        fine[0, :, :4] = False                            # (position 5 of the first sequence)
+        fine[1] = False                                   # (positions from 6 on of the second)
+        fine = fine.view(B * nodes, hq)
+        close(got[fine.to(dev)], want.view(B * nodes, hq, d)[fine], tol.view(B * nodes, hq, d)[fine])
