@@ -476,6 +476,8 @@ def _addr(t: Optional[torch.Tensor]):
 
 
 def _i32(t, n, what: str) -> None:
+    if t is None:
+        raise SpacerError(f"{what}: expected {n} contiguous int32 values, got None")
     if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
         raise SpacerError(f"{what}: expected {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
 
@@ -562,6 +564,8 @@ def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, rows: torch.Tenso
 
 def _kv_lengths(t: torch.Tensor, n: int, what: str) -> int:
     """1 when ``t`` holds one length per sequence, 0 when one for all of them."""
+    if t is None:
+        raise SpacerError(f"{what}: expected 1 or {n} contiguous int32 values, got None")
     m = t.numel()
     if t.dtype != torch.int32 or not (m == n or m == 1) or not t.is_contiguous():
         raise SpacerError(f"{what}: expected 1 or {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}")
