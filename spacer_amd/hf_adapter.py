@@ -74,10 +74,11 @@ class SpacerModel:
         n = int(getattr(gc, "num_return_sequences", 1) or 1)
         do_sample = bool(getattr(gc, "do_sample", False))
         top_k = getattr(gc, "top_k", None)
+        penalty = getattr(gc, "repetition_penalty", None)            # (0 goes on, to be refused as HF refuses it)
         sp = SamplingParams(max_new_tokens=int(gc.max_new_tokens), top_k=(int(top_k) if top_k else (0 if do_sample else 1)) if do_sample else 1,
                             top_p=float(getattr(gc, "top_p", 1.0) or 1.0) if do_sample else 1.0,
                             temperature=float(getattr(gc, "temperature", 1.0) or 1.0), seed=self.seed + 7919 * self._calls,
-                            era_rule=self.era_rule, repetition_penalty=float(getattr(gc, "repetition_penalty", None) or 1.0))
+                            era_rule=self.era_rule, repetition_penalty=1.0 if penalty is None else float(penalty))
         if sp.top_k == 0:
             sp.top_k = self.cfg.vocab                                # HF top_k=None: no top-k cut
         self._calls += 1

@@ -23,3 +23,22 @@ def test_missing_lengths_and_rows_are_refused():
                  lambda: K.decode_qkv_finish_cache(torch.zeros(2, 8 * 64), None, torch.zeros(2, 64), torch.zeros(2, 64), torch.zeros(2, 256, dtype=BF), cache, None, 4)):
         with pytest.raises(K.SpacerError, match="int32"):
             call()
+
+
+def test_adapter_passes_the_repetition_penalty_on():
+    """generation_config.repetition_penalty as given, None or absent as 1; 0 reaches the rules, which refuse it."""
+    from spacer_amd.hf_adapter import SpacerModel
+    from spacer_amd.rollout import SamplingParams, _LogitRules
+    seen = []
+    model = object.__new__(SpacerModel)
+    model.__dict__.update(seed=0, _calls=0, era_rule=False, device="cpu", cfg=SimpleNamespace(vocab=100), _pixels=lambda kw: (None, None),
+                          roll=SimpleNamespace(generate=lambda prompts, n, sp: seen.append(sp) or torch.zeros(n, 2, dtype=torch.int64)))
+    ids = torch.arange(4)[None]
+    for given, want in (({}, 1.0), (dict(repetition_penalty=None), 1.0), (dict(repetition_penalty=1.3), 1.3), (dict(repetition_penalty=0.0), 0.0), (dict(repetition_penalty=0), 0.0)):
+        out = model.generate(input_ids=ids, generation_config=SimpleNamespace(max_new_tokens=2, num_return_sequences=3, do_sample=True, top_k=5, **given))
+        assert out.shape == (3, 6) and seen[-1].repetition_penalty == want, given
+        if want == 0.0:
+            assert _LogitRules.wanted(seen[-1])
+            with pytest.raises(ValueError, match="repetition"):
+                _LogitRules(seen[-1], [], [1], 100, 7, "cpu")
+    assert not _LogitRules.wanted(SamplingParams())
