@@ -483,7 +483,8 @@ int spacer_attn_fwd_pair(const void* q_hi, const void* q_lo, const void* k_hi, c
  *   SPACER_KV_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| / scale <= 448
  *   SPACER_KV_INT8  two's complement codes -127 .. 127; scale = max|x| / 127 in fp32, ties of x / scale to even
  * A row with a NaN or an infinity gets scale NaN and codes 0 (it stands for NaN).  Scales of e4m3 rows that a caller makes by other means
- * must be powers of two (of 2^-126 or more) or 0 as well: to spacer_attn_cache a row with any other scale is a row of NaN.  Rows may share memory (an expanded view) in a cache that is only read.
+ * must be powers of two (of 2^-126 or more) or 0 as well: to spacer_attn_cache a row with any other scale is a row of NaN.  Rows may share memory (an expanded view, k and v of one
+ * tensor) in a cache that is only read; the writers refuse it.
  * ---------------------------------------------------------------------------------------------- */
 enum spacer_kv_format { SPACER_KV_BF16 = 0, SPACER_KV_E4M3 = 1, SPACER_KV_INT8 = 2 };
 typedef struct spacer_kv_cache {

@@ -269,6 +269,38 @@ static int check_target(const spacer_kv_cache* c, const char* who) {
     return SPACER_OK;
 }
 
+// Does a row of k meet a row of v?  With every dimension at least as wide as all below it (`apart`), v's first number lies at delta from k's and a row pair at
+// delta - sum_j d_j s_j, |d_j| < n_j: a dimension's d_j is the quotient of what the wider ones left, or one more.
+static bool meet(long delta, const long* s, const long* n, int dims, long extent) {
+    if (dims == 0) return delta > -extent && delta < extent;
+    long q = delta / s[0];
+    if (delta % s[0] < 0) --q;
+    for (long d = q; d <= q + 1; ++d)
+        if (d > -n[0] && d < n[0] && meet(delta - d * s[0], s + 1, n + 1, dims - 1, extent)) return true;
+    return false;
+}
+static bool pair_apart(const spacer_kv_cache* c, const void* k, const void* v, long s0, long s1, long s2, long extent, long size) {
+    long all[3] = {s0, s1, s2}, count[3] = {c->n_seq, c->kv_heads, c->capacity}, s[3], n[3];
+    int dims = 0;
+    for (;;) {                                            // dimensions by falling stride, in bytes
+        int at = -1;
+        for (int j = 0; j < 3; ++j)
+            if (count[j] > 1 && (at < 0 || all[j] > all[at])) at = j;
+        if (at < 0) break;
+        s[dims] = all[at] * size; n[dims++] = count[at];
+        count[at] = 1;
+    }
+    return !meet((long)((uintptr_t)v - (uintptr_t)k), s, n, dims, extent * size);
+}
+// ... of a cache that check_target has passed, where something is written
+static int check_pair(const spacer_kv_cache* c, const char* who) {
+    SP_REQUIRE(pair_apart(c, c->k, c->v, c->stride_seq, c->stride_head, c->stride_pos, c->head_dim, c->format == KV_BF16 ? 2 : 1), SPACER_EINVAL,
+               "%s: rows of k and v share memory", who);
+    SP_REQUIRE(c->format == KV_BF16 || pair_apart(c, c->k_scale, c->v_scale, c->scale_stride_seq, c->scale_stride_head, c->scale_stride_pos, 1, 4), SPACER_EINVAL,
+               "%s: scales of k and v share memory", who);
+    return SPACER_OK;
+}
+
 KvView spacer_kv_view(const spacer_kv_cache* c) {
     return KvView{(char*)c->k, (char*)c->v, c->k_scale, c->v_scale, c->stride_seq, c->stride_head, c->stride_pos, c->scale_stride_seq,
                   c->scale_stride_head, c->scale_stride_pos, c->n_seq, c->capacity};
@@ -288,6 +320,7 @@ extern "C" int spacer_kv_write(const spacer_kv_cache* c, const void* k, const vo
     if (int rc = check_target(c, "kv_write")) return rc;
     SP_REQUIRE(n_src >= 0 && rows, SPACER_EINVAL, "kv_write: rows required, n_src >= 0");
     if (n_src == 0) return SPACER_OK;
+    if (int rc = check_pair(c, "kv_write")) return rc;
     if (int rc = check_source(k, v, ld, "kv_write")) return rc;
     const long per_seq = (long)c->capacity * c->kv_heads;
     const unsigned chunks = row_chunks(c->n_seq, per_seq, 4 * (512 / c->head_dim) * RU);
@@ -306,6 +339,7 @@ extern "C" int spacer_kv_append(const spacer_kv_cache* c, const void* k, const v
     if (int rc = check_target(c, "kv_append")) return rc;
     SP_REQUIRE(N >= 0 && len, SPACER_EINVAL, "kv_append: lengths required, N >= 0");
     if (N == 0) return SPACER_OK;
+    if (int rc = check_pair(c, "kv_append")) return rc;
     if (int rc = check_source(k, v, ld, "kv_append")) return rc;
     const long per_seq = (long)N * c->kv_heads;
     const unsigned chunks = row_chunks(c->n_seq, per_seq, 4 * (512 / c->head_dim) * RU);
@@ -343,6 +377,7 @@ extern "C" int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, co
                                               const spacer_kv_cache* c, const int* tail_len, int len_per_seq, const float* rowss, float* rowss_zero,
                                               int norm_cols, float eps, int Hq, spacer_stream_t stream) {
     if (int rc = check_target(c, "decode_qkv_finish_cache")) return rc;
+    if (int rc = check_pair(c, "decode_qkv_finish_cache")) return rc;
     const int B = c->n_seq, heads = Hq + 2 * c->kv_heads;
     SP_REQUIRE(acc32 && cos_t && sin_t && q_out && tail_len, SPACER_EINVAL, "decode_qkv_finish_cache: missing operand");
     SP_REQUIRE(Hq > 0, SPACER_EINVAL, "decode_qkv_finish_cache: Hq = %d", Hq);

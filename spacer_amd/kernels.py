@@ -495,7 +495,7 @@ class KVCache:
         int8            scale = max|row| / 127, codes -127 .. 127, ties of x / scale to even
     A row that holds a NaN or an infinity gets scale NaN.  (e4m3 scales made elsewhere must be powers of two or 0 too: to ``attn_cache`` a
     row with another one is a row of NaN.)  The object only describes the
-    tensors (and keeps them alive); expanded views can be read, not written."""
+    tensors (and keeps them alive); expanded views, and k and v that share rows, can be read, not written."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "kv_heads", "capacity", "head_dim", "dtype", "device", "_c", "_ref", "_shape")
 

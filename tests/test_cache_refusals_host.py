@@ -42,3 +42,72 @@ def test_adapter_passes_the_repetition_penalty_on():
             with pytest.raises(ValueError, match="repetition"):
                 _LogitRules(seen[-1], [], [1], 100, 7, "cpu")
     assert not _LogitRules.wanted(SamplingParams())
+
+
+EINVAL = -1
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    return _lib.load()
+
+
+def described(shape, strides, sstrides, fmt, delta, sdelta):
+    """A cache whose v (v_scale) lies delta elements (sdelta floats) behind its k (k_scale); the memory is never touched."""
+    size, base = 2 if fmt == _lib.SPACER_KV_BF16 else 1, 1 << 40
+    return _lib.KvCache(format=fmt, n_seq=shape[0], kv_heads=shape[1], capacity=shape[2], head_dim=shape[3], k=base, v=base + delta * size,
+                        k_scale=None if size == 2 else 2 * base, v_scale=None if size == 2 else 2 * base + 4 * sdelta,
+                        stride_seq=strides[0], stride_head=strides[1], stride_pos=strides[2],
+                        scale_stride_seq=sstrides[0], scale_stride_head=sstrides[1], scale_stride_pos=sstrides[2])
+
+
+def refusal(lib, c):
+    """What the writers say of a cache: the sources are refused last (before any launch), so an otherwise good call names them."""
+    p, said = 0x10002, set()
+    for rc in (lib.spacer_kv_write(C.byref(c), p, p, 1024, 4, p, None), lib.spacer_kv_append(C.byref(c), p, p, 1024, 1, p, 0, None)):
+        assert rc == EINVAL
+        said.add(lib.spacer_last_error().decode().split(": ", 1)[1])
+    assert lib.spacer_decode_qkv_finish_cache(None, None, None, None, None, C.byref(c), None, 0, None, None, 0, 0.0, 4, None) == EINVAL
+    last = lib.spacer_last_error().decode()
+    assert len(said) == 1
+    said = said.pop()
+    assert ("share memory" in said) == ("share memory" in last), (said, last)
+    return said
+
+
+# (sequences, heads, positions, D) with strides in elements of two layouts, and of rows spread over wider memory
+LAYOUTS = [((2, 3, 5, 64), (3 * 5 * 64, 5 * 64, 64)), ((2, 3, 5, 64), (5 * 3 * 64, 64, 3 * 64)), ((3, 2, 4, 128), (4096, 2048, 256)), ((1, 1, 7, 64), (0, 0, 192)), ((3, 1, 1, 128), (384, 0, 0)),
+           ((1, 1, 1, 64), (0, 0, 0))]
+
+
+@pytest.mark.parametrize("fmt", [_lib.SPACER_KV_BF16, _lib.SPACER_KV_INT8])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_rows_of_k_and_v_are_apart(lib, layout, fmt):
+    """Against the sets of addresses: every distance between k and v up to beyond the cache's end, to either side."""
+    shape, strides = layout
+    n, h, cap, d = shape
+    starts = {a * strides[0] + b * strides[1] + c * strides[2] for a in range(n) for b in range(h) for c in range(cap)}
+    span, step = max(starts) + d, 16 // (2 if fmt == _lib.SPACER_KV_BF16 else 1)
+    near = {x - y for x in starts for y in starts}
+    for delta in range(-span - 32, span + 33):
+        if delta % step or delta == 0:
+            continue
+        overlap = any(-d < delta - x < d for x in near)
+        c = described(shape, strides, (1 << 20, 1 << 15, 1), fmt, delta, 1 << 30)
+        assert refusal(lib, c) == ("rows of k and v share memory" if overlap else "source rows must start at multiples of 16 bytes"), delta
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_scales_of_k_and_v_are_apart(lib, layout):
+    shape, strides = layout
+    n, h, cap, _ = shape
+    s = tuple(x // 64 for x in strides)
+    starts = {a * s[0] + b * s[1] + c * s[2] for a in range(n) for b in range(h) for c in range(cap)}
+    for delta in range(-max(starts) - 3, max(starts) + 4):
+        if delta == 0:
+            continue
+        overlap = any((x + delta) in starts for x in starts)
+        c = described(shape, strides, s, _lib.SPACER_KV_INT8, 1 << 35, delta)
+        assert refusal(lib, c) == ("scales of k and v share memory" if overlap else "source rows must start at multiples of 16 bytes"), delta
