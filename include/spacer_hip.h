@@ -510,7 +510,7 @@ int spacer_kv_append(const spacer_kv_cache* cache, const void* k, const void* v,
  * cache stands for; with len (int32 [n_seq], or NULL) the positions at and behind len[s] are zero. */
 int spacer_kv_read(const spacer_kv_cache* cache, const int* len, void* k_out, void* v_out, int out_f32, spacer_stream_t stream);
 /* spacer_decode_qkv_finish (rowss NULL) / spacer_decode_qkv_finish_normed with K and V going to position tail_len of the cache's sequences
- * (cache->n_seq = the batch), rounded to bf16 first, then to the cache's format as spacer_kv_append rounds. */
+ * (cache->n_seq = the batch), rounded to bf16 first, then to the cache's format as spacer_kv_append rounds.  rowss_zero is not rowss. */
 int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, const float* cos_t, const float* sin_t, void* q_out,
                                    const spacer_kv_cache* cache, const int* tail_len, int len_per_seq, const float* rowss, float* rowss_zero,
                                    int norm_cols, float eps, int Hq, spacer_stream_t stream);

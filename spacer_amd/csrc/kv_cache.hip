@@ -382,6 +382,8 @@ extern "C" int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, co
     SP_REQUIRE(acc32 && cos_t && sin_t && q_out && tail_len, SPACER_EINVAL, "decode_qkv_finish_cache: missing operand");
     SP_REQUIRE(Hq > 0, SPACER_EINVAL, "decode_qkv_finish_cache: Hq = %d", Hq);
     SP_REQUIRE(!rowss || norm_cols > 0, SPACER_EINVAL, "decode_qkv_finish_cache: norm_cols = %d", norm_cols);
+    // (one workgroup clears rowss_zero while the others still read rowss)
+    SP_REQUIRE(!rowss || !rowss_zero || rowss + B <= rowss_zero || rowss_zero + B <= rowss, SPACER_EINVAL, "decode_qkv_finish_cache: rowss_zero overlaps rowss");
     SP_REQUIRE(!rowss_zero || B <= 256, SPACER_EINVAL, "decode_qkv_finish_cache: at most 256 rows with rowss_zero, got %d", B);
     const dim3 grid(cdiv((long)B * heads, 4)), block(256);
 #define CALL(F)                                                                                                                                     \

@@ -111,3 +111,18 @@ def test_scales_of_k_and_v_are_apart(lib, layout):
         overlap = any((x + delta) in starts for x in starts)
         c = described(shape, strides, s, _lib.SPACER_KV_INT8, 1 << 35, delta)
         assert refusal(lib, c) == ("scales of k and v share memory" if overlap else "source rows must start at multiples of 16 bytes"), delta
+
+
+def test_row_sums_to_clear_are_not_those_to_read(lib):
+    """decode_qkv_finish_cache clears rowss_zero while it reads rowss."""
+    p, rows = 0x10000, 300                               # (too many rows to clear: an otherwise good call ends there, before any launch)
+    c = described((rows, 1, 1, 64), (64, 0, 0), (1, 0, 0), _lib.SPACER_KV_INT8, 1 << 30, 1 << 30)
+
+    def finish(rowss, rowss_zero):
+        assert lib.spacer_decode_qkv_finish_cache(p, None, p, p, p, C.byref(c), p, 0, rowss, rowss_zero, 64, 0.0, 4, None) == EINVAL
+        return lib.spacer_last_error().decode()
+    for other in (p, p + 4, p + 4 * (rows - 1), p - 4 * (rows - 1)):
+        assert "overlaps" in finish(p, other)
+    for other in (p + 4 * rows, p - 4 * rows):
+        assert "at most 256" in finish(p, other)
+    assert "at most 256" in finish(None, p)
