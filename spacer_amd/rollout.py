@@ -90,11 +90,13 @@ class SamplingParams:
 
 
 class _LayerCaches:
-    """One kernels.KVCache per decoder layer over common allocations [layers, n_seq, kv_heads, capacity, head_dim]."""
+    """One kernels.KVCache per decoder layer over common allocations [layers, n_seq, kv_heads, capacity, head_dim].  Slots behind a sequence's length
+    may hold anything (attention reads none of them), so the prompts' caches are not cleared."""
 
-    def __init__(self, layers: int, n_seq: int, capacity: int, kv_heads: int, head_dim: int, dtype: str, device):
-        self.codes = [torch.zeros(layers, n_seq, kv_heads, capacity, head_dim, device=device, dtype=torch.uint8).view(K.KV_DTYPES[dtype]) for _ in range(2)]
-        self.scales = [torch.zeros(layers, n_seq, kv_heads, capacity, device=device, dtype=F32) for _ in range(2)]
+    def __init__(self, layers: int, n_seq: int, capacity: int, kv_heads: int, head_dim: int, dtype: str, device, clear: bool = True):
+        new = torch.zeros if clear else torch.empty
+        self.codes = [new(layers, n_seq, kv_heads, capacity, head_dim, device=device, dtype=torch.uint8).view(K.KV_DTYPES[dtype]) for _ in range(2)]
+        self.scales = [new(layers, n_seq, kv_heads, capacity, device=device, dtype=F32) for _ in range(2)]
         self.layers = [self.part(i, 0, n_seq) for i in range(layers)]
         self.capacity = capacity
 
@@ -459,7 +461,8 @@ class RolloutEngine:
         if n_keep == 0:
             self.prefill_tape_bytes = 0
         self.prefill_tape_prompts = n_keep               # (of len(prompts), counted from the front)
-        narrow = None if sp.kv_cache == "bf16" else _LayerCaches(cfg.layers, nP, max(p.ids.numel() for p in prompts), cfg.kv_heads, cfg.head_dim, sp.kv_cache, dev)
+        narrow = None if sp.kv_cache == "bf16" else _LayerCaches(cfg.layers, nP, max(p.ids.numel() for p in prompts), cfg.kv_heads, cfg.head_dim, sp.kv_cache, dev,
+                                                                        clear=False)
         if n_keep in (0, len(prompts)):
             pk, pv, first_logits, plen, pos_base = self._prefill(prompts, sp.era_rule, keep_tape=n_keep > 0, out=None if narrow is None else (narrow, None, 0))
         else:
