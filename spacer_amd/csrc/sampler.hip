@@ -11,7 +11,7 @@
 namespace {
 
 constexpr int SNT = 1024;
-constexpr int CAP = 1024;    // candidate capacity (top_k <= CAP; ties beyond CAP are dropped)
+constexpr int CAP = 1024;    // candidate capacity (top_k <= CAP; of ties beyond CAP those of the lowest indices stay)
 
 // The least key of a logit above -infinity.  Forbidden tokens are no candidates: where fewer than top_k tokens are allowed they would be ties of the
 // top_k-th largest logit, and more of them than CAP would push allowed tokens out of the list.
@@ -190,12 +190,28 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
     const bool none = ncand == 0;                         // every token forbidden: some token, as there is no answer
     if (none) gather(bound);
     if (ncand > CAP) {
-        const uint32_t kth = kth_key(val, vocab, top_k);
-        gather(none ? kth : max(kth, KEY_FINITE));
+        const uint32_t exact = kth_key(val, vocab, top_k), kth = none ? exact : max(exact, KEY_FINITE);
+        gather(kth);
+        const bool crowd = ncand > CAP;                   // more ties of the top_k-th logit than the list takes
+        __syncthreads();
+        if (crowd) {
+            // which of them the atomics of gather() would leave in the list depends on the order of the waves: the lowest indices stay, found by a
+            // select over the ties' indices (as positive floats that fall with the index)
+            gather(kth + 1);                              // the logits above, fewer than top_k
+            const int room = CAP - ncand;
+            auto tie = [&](int i) -> float { return okey(val(i)) == kth ? __uint_as_float(0x7f000000u - (uint32_t)i) : -INFINITY; };
+            const uint32_t last = kth_key(tie, vocab, room);
+            for (int i = tid; i < vocab; i += SNT) {
+                if (okey(tie(i)) < last) continue;
+                const int slot = atomicAdd(&ncand, 1);
+                cval[slot] = val(i); cidx[slot] = i;
+            }
+            __syncthreads();
+        }
         trimmed_exactly = true;
     }
     }
-    const int n = min(ncand, CAP);   // (ties beyond CAP are dropped)
+    const int n = min(ncand, CAP);
     int np2 = 1;
     while (np2 < n) np2 <<= 1;
     for (int i = n + tid; i < np2; i += SNT) { cval[i] = -INFINITY; cidx[i] = 0x7fffffff; }
