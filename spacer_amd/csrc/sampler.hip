@@ -19,7 +19,8 @@ constexpr uint32_t KEY_FINITE = 0x00800000u;
 
 // A NaN logit is a forbidden one.  No comparison places it: the sort would leave it (or a filler of the sort) anywhere, a top_k-th value of NaN would
 // keep no candidate and a negative NaN lies below -infinity's key, so that no candidate would be found at all -- the token would then be read from
-// in front of the list.  With NaN as -infinity every row has a candidate: what is above -infinity, or (nothing is) all of the row.
+// in front of the list.  Every row has a candidate: what is above -infinity, or (nothing is) the first tokens.  The passes over the row take maxima, which
+// pass a NaN by, and look for one only in what is about to become a candidate (in every logit: 37 instead of 33 us at 8 rows, one workgroup per row).
 __device__ __forceinline__ float never_nan(float x) { return x == x ? x : -INFINITY; }
 
 __device__ __forceinline__ uint32_t okey(float x) {
@@ -134,16 +135,16 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
         return;
     }
     const float* row = logits + (long)b * ld;
-    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : never_nan(raw * inv_temp); };
-    auto val = [&](int i) -> float { return fix(row[i], i); };
+    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
+    auto val = [&](int i) -> float { return never_nan(fix(row[i], i)); };
     const bool vec_ok = (ld % 4 == 0) && (((uintptr_t)logits & 15) == 0);
 
     auto kth_key = [&](auto&& load, int count, int k) -> uint32_t { return kth_key_fn(load, count, k, hist, sel_bin, sel_k); };
-    auto gather = [&](uint32_t thr) {
+    auto gather = [&](uint32_t thr) {                       // (thr > the key of -infinity: a NaN's place)
         if (tid == 0) ncand = 0;
         __syncthreads();
         auto consider = [&](float x, int i) {
-            if (okey(x) >= thr) {
+            if (okey(x) >= thr && x == x) {
                 const int slot = atomicAdd(&ncand, 1);
                 if (slot < CAP) { cval[slot] = x; cidx[slot] = i; }
             }
@@ -188,9 +189,14 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
     __syncthreads();
     gather(max(bound, KEY_FINITE));
     const bool none = ncand == 0;                         // every token forbidden: some token, as there is no answer
-    if (none) gather(bound);
+    if (none) {
+        if (tid < min(vocab, CAP)) { cval[tid] = -INFINITY; cidx[tid] = tid; }
+        __syncthreads();
+        if (tid == 0) ncand = min(vocab, CAP);
+        __syncthreads();
+    }
     if (ncand > CAP) {
-        const uint32_t exact = kth_key(val, vocab, top_k), kth = none ? exact : max(exact, KEY_FINITE);
+        const uint32_t kth = max(kth_key(val, vocab, top_k), KEY_FINITE);
         gather(kth);
         const bool crowd = ncand > CAP;                   // more ties of the top_k-th logit than the list takes
         __syncthreads();
@@ -305,7 +311,7 @@ __global__ __launch_bounds__(SNT) void sample_partmax_kernel(const float* __rest
     if (sl == 0 && tid == 0) pre_n[b] = 0;
     if (finished && finished[b]) return;
     const float* row = logits + (long)b * ld;
-    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : never_nan(raw * inv_temp); };
+    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
     const int n4 = vocab >> 2, per = (n4 + S - 1) / S, q0 = sl * per, q1 = min(n4, q0 + per);
     float lmax = -INFINITY;
     for (int i4 = q0 + tid; i4 < q1; i4 += SNT) {
@@ -334,9 +340,9 @@ __global__ __launch_bounds__(SNT) void sample_gather_kernel(const float* __restr
     __syncthreads();
     const uint32_t thr = max(kth_key_fn([&](int i) { return mx[i]; }, S * SNT, top_k, hist, sel_bin, sel_k), KEY_FINITE);
     const float* row = logits + (long)b * ld;
-    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : never_nan(raw * inv_temp); };
+    auto fix = [&](float raw, int i) -> float { return (suppress_eos && i == eos) ? -INFINITY : raw * inv_temp; };
     auto consider = [&](float x, int i) {
-        if (okey(x) >= thr) {
+        if (okey(x) >= thr && x == x) {
             const int slot = atomicAdd(&nloc, 1);
             if (slot < CAP) { lval[slot] = x; lidx[slot] = i; }
         }
