@@ -388,7 +388,7 @@ int spacer_decode_embed(const int64_t* ids, const void* table, float* out, int B
                         spacer_stream_t stream);
 /* Round 6: spacer_sample_top_p / spacer_sample_top_p_step_ws with a workspace of spacer_sample_workspace_bytes(B, vocab) bytes (16-byte
  * aligned, scratch, no initialisation) run the two passes over a row's logits with several workgroups per row when the batch alone cannot
- * fill the chip (B < 256 rows of >= 64 K logits): 32.6 / 39.4 / 46.9 / 58.3 -> 30.4 / 30.7 / 34.3 / 47.2 us per call at 8 / 12 / 64 / 128 rows
+ * fill the chip (B < 256 rows of >= 64 K logits): 34.8 / 41.3 / 47.9 / 58.9 -> 31.7 / 32.0 / 35.1 / 47.7 us per call at 8 / 12 / 64 / 128 rows
  * (scripts/probes/sampler_time.py; what remains is the select / sort / draw chain of three dependent launches, not the passes).  Same token for the same logits and counter as the
  * one-workgroup-per-row form (the candidate list is sorted by (value, index) before the exact top-k trim); workspace NULL = that form. */
 int spacer_sample_top_p_step_ws(const float* logits, long ld, int B, int vocab, int top_k, float top_p, float temperature, uint64_t seed,

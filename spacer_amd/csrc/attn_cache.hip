@@ -17,7 +17,7 @@
 // The waves' (O, m, l) are joined through LDS, the ranges' through fp32 records and a second small launch.  Short contexts take one launch of 8 waves
 // per workgroup that walk the prompt's and the sequence's keys and write the output themselves (plan_attn).
 // Measured (kernels alone): 2 x 12 heads over 220 int8 positions 6.2 us; 8 x 8 rollouts x 28 heads over 1391 + 300 e4m3 positions 14 us, over 16384 + 700 of
-// int8 42 + 5 (join); 8 trees of 13 over 2311 + 211 bf16 positions 16 + 4; 32 trees of 32 over 5498 + 333 e4m3 positions of D = 64 50 + 5.  Many columns per
+// int8 42 + 5 (join); 8 trees of 13 over 2311 + 211 bf16 positions 16 + 4; 32 trees of 32 over 5498 + 333 e4m3 positions of D = 64 52 + 5.  Many columns per
 // key are bound by the softmax's and the conversions' VALU work (about 160 operations and 16 exponentials beside 18 products a tile of 32 x 32, D = 64), few by
 // the latency of a tile's rows.
 #include <math.h>
@@ -634,8 +634,9 @@ struct AttnPlan {
 //   more                  13.4 | 14.1 us at 400, but 10 to 20 % slower from 700 on at 512: a second round of workgroups
 // 16 columns per workgroup while these are no more than the CUs (narrow 256: 14.2 us, with 32 columns 16.8; narrow 384, D = 64: 13.6 | 11.9).
 // Others: of the widths (16 or 32 columns) and numbers of key ranges (sa, sb) the one whose estimate (us) is least: 512 workgroups run at once (two per CU), one
-// costs a constant and its 32-key tiles per wave, a record of a column its bytes.  The constants were fitted to 2400 launches of 96 settings (1 to 16
-// prompts of equal and of falling lengths, 4 to 4096 columns, 1300 to 30000 positions, all formats): the choice is 3.5 % behind the best of them in the mean.
+// costs a constant and its 32-key tiles per wave, a record of a column its bytes.  The constants were fitted to 2964 launches of 96 settings (1 to 16
+// prompts of equal and of falling lengths, 4 to 4096 columns, 1300 to 30000 positions, all formats): the choice is 3.6 % behind the best of them in the mean,
+// 15 % at worst.
 // (8 waves per workgroup here too: level with 4 for single long prompts, 2 to 20 % behind elsewhere, so this form has 4.)
 AttnPlan plan_attn(const spacer_kv_cache* prompt, const spacer_kv_cache* tail, int rows, int B, int N, int Hq) {
     const spacer_kv_cache* c = prompt ? prompt : tail;

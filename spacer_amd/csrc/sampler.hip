@@ -295,7 +295,7 @@ __global__ __launch_bounds__(SNT) void sample_kernel(const float* __restrict__ l
 
 // ---- wide form (round 6): the two passes over a row's logits by S workgroups per row instead of one.  At decode batch sizes (8 ... 128 rows of
 // 152 064 logits) one workgroup per row leaves most CUs idle and each reads 1.2 MB alone.  Measured (scripts/probes/sampler_time.py):
-// 32.6 / 39.4 / 46.9 / 58.3 us per call at 8 / 12 / 64 / 128 rows in that form, 30.4 / 30.7 / 34.3 / 47.2 us in this one -- the passes shrink, the
+// 34.8 / 41.3 / 47.9 / 58.9 us per call at 8 / 12 / 64 / 128 rows in that form, 31.7 / 32.0 / 35.1 / 47.7 us in this one -- the passes shrink, the
 // select / sort / draw chain (now three dependent launches) stays.  Here
 //   sample_partmax_kernel   (B x S workgroups)  per-thread maxima of a slice of the row -> pmax[b][S x 1024]
 //   sample_gather_kernel    (B x S workgroups)  bound = top_k-th largest of the row's S x 1024 maxima (each is a logit of the row, so
