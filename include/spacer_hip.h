@@ -483,8 +483,8 @@ int spacer_attn_fwd_pair(const void* q_hi, const void* q_lo, const void* k_hi, c
  *   SPACER_KV_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| / scale <= 448
  *   SPACER_KV_INT8  two's complement codes -127 .. 127; scale = max|x| / 127 in fp32, ties of x / scale to even
  * A row with a NaN or an infinity gets scale NaN and codes 0 (it stands for NaN).  Scales of e4m3 rows that a caller makes by other means
- * must be powers of two (of 2^-126 or more) or 0 as well: to spacer_attn_cache a row with any other scale is a row of NaN.  Rows may share memory (an expanded view, k and v of one
- * tensor) in a cache that is only read; the writers refuse it.
+ * must be powers of two (of 2^-126 or more) or 0 as well: to spacer_attn_cache a row with any other scale is a row of NaN.  Rows may share
+ * memory (an expanded view, k and v of one tensor) in a cache that is only read; the writers refuse it.
  * ---------------------------------------------------------------------------------------------- */
 enum spacer_kv_format { SPACER_KV_BF16 = 0, SPACER_KV_E4M3 = 1, SPACER_KV_INT8 = 2 };
 typedef struct spacer_kv_cache {
@@ -521,8 +521,9 @@ int spacer_decode_qkv_finish_cache(float* acc32, const void* bias, const float* 
  *   the positions [0, tail_len[b]) of sequence b in `tail` (NULL: none), and
  *   the nodes j whose bit j is set in tree[b * tree_per_seq * N + i] (int64; NULL: j <= i), node j at position tail_len[b] + j of `tail`.
  * Prompt p owns the sequences [row0[p], row0[p + 1]) (int32 [n_prompts + 1] on the device, ascending; `rows` = as many as a prompt usually has:
- * what the launch is cut for, more are served in a second round), or with row0 NULL [p * rows, (p + 1) * rows).  Lengths are clamped to the caches.  A node that sees nothing, or
- * only keys whose score is -infinity, gets zeros; a NaN that it sees (query, key or value row) gives NaN.
+ * what the launch is cut for, more are served in a second round), or with row0 NULL [p * rows, (p + 1) * rows).  Lengths are clamped to
+ * the caches.  A node that sees nothing, or only keys whose score is -infinity, gets zeros; a NaN that it sees (query, key or value row)
+ * gives NaN.
  * scale > 0.  o bf16 [B * N, Hq * head_dim] contiguous.  prompt and tail share format, kv_heads and head_dim; tail->n_seq = B.
  * workspace: spacer_attn_cache_workspace_bytes(...) bytes of device memory, 16-byte aligned, no initialisation; the cache structs may be NULL
  * there as in the call.  Launches that share a workspace must be ordered on one stream. */
